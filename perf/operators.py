@@ -1,0 +1,496 @@
+"""Timed cases of the cache operators: appending rotated keys and values to a paged cache,
+attention over an e4m3 cache, the choice of cache blocks by a bound of their keys, and the
+attention over the chosen blocks.
+
+  append  append_kv: queries and keys rotated, keys and values into their cache slots, bounds
+          of the blocks that became full
+  fp8     fp8_decode: one token per sequence over its whole e4m3 cache
+  select  select_blocks: the blocks a sparse decode step reads, per sequence and kv head
+  sparse  sparse_decode: one token per sequence over the listed blocks
+
+``prepare`` builds what a serving loop has in hand (cache, tables, rotation table, plan),
+``run`` makes one pass, with ``own`` through the package, else in elementary torch operations.
+"""
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+PAGE, BLOCK = 256, 64
+DEV = "cuda"
+E4M3, E4M3_MAX = torch.float8_e4m3fn, 448.0
+TYPES = {"bf16": torch.bfloat16, "e4m3": E4M3}
+
+# (query heads, kv heads, head dim) of the benchmark, the engine tests and the edge batches
+GEOMETRIES = [(16, 4, 256), (32, 8, 128), (32, 4, 256), (16, 16, 64), (16, 8, 128), (8, 2, 128)]
+
+
+def listed():
+    return [
+        # one user's decode step of the decoder with partial rotation: latency
+        {"name": "append_one", "kind": "append", "cache": "bf16", "batch": 1, "hq": 16, "hkv": 4,
+         "dim": 256, "half": 32, "interleaved": False, "low": 1, "high": 1, "padded": 0},
+        # a serving batch's decode step, a graph bucket with unused rows, 8-bit cache
+        {"name": "append_step_b64_e4m3", "kind": "append", "cache": "e4m3", "batch": 64, "hq": 32,
+         "hkv": 8, "dim": 128, "half": 64, "interleaved": False, "low": 1, "high": 1, "padded": 5},
+        # four prompts of ragged lengths packed into one prefill call
+        {"name": "append_prompts", "kind": "append", "cache": "bf16", "batch": 4, "hq": 32,
+         "hkv": 8, "dim": 128, "half": 64, "interleaved": False, "low": 300, "high": 4001,
+         "padded": 0},
+        # one long prompt of odd length, neighbouring elements rotated, multi-head, 8-bit cache
+        {"name": "append_prompt_mha64_e4m3", "kind": "append", "cache": "e4m3", "batch": 1,
+         "hq": 16, "hkv": 16, "dim": 64, "half": 32, "interleaved": True, "low": 2049,
+         "high": 2049, "padded": 0},
+        # one sequence, a short context: latency
+        {"name": "fp8_ctx2064", "kind": "fp8", "batch": 1, "hq": 16, "hkv": 4, "dim": 256,
+         "low": 2064, "high": 2064},
+        # a serving batch of a multi-head model, lengths spread up to 4096 tokens
+        {"name": "fp8_b128_mha64", "kind": "fp8", "batch": 128, "hq": 16, "hkv": 16, "dim": 64,
+         "low": 1, "high": 4096},
+        # 64 long-context sequences of a grouped-query model
+        {"name": "fp8_b64_gqa128", "kind": "fp8", "batch": 64, "hq": 32, "hkv": 8, "dim": 128,
+         "low": 1, "high": 32768},
+        # one user at a long context: every block scored, an eighth kept
+        {"name": "select_ctx32768", "kind": "select", "batch": 1, "hq": 16, "hkv": 4, "dim": 256,
+         "low": 32768, "high": 32768, "kept": 64},
+        # the same for 64 sequences of ragged lengths, some of fewer blocks than are kept
+        {"name": "select_b64_gqa128", "kind": "select", "batch": 64, "hq": 32, "hkv": 8,
+         "dim": 128, "low": 1, "high": 32768, "kept": 64},
+        # the attention over those blocks, one user
+        {"name": "sparse_ctx32768", "kind": "sparse", "cache": "bf16", "batch": 1, "hq": 16,
+         "hkv": 4, "dim": 256, "low": 32768, "high": 32768, "kept": 64},
+        # and the batch
+        {"name": "sparse_b64_gqa128", "kind": "sparse", "cache": "bf16", "batch": 64, "hq": 32,
+         "hkv": 8, "dim": 128, "low": 1, "high": 32768, "kept": 64},
+        # eight query heads a kv head, 8-bit cache, an odd number of blocks
+        {"name": "sparse_b17_gqa256_e4m3", "kind": "sparse", "cache": "e4m3", "batch": 17,
+         "hq": 32, "hkv": 4, "dim": 256, "low": 100, "high": 20001, "kept": 37},
+    ]
+
+
+def _log(rng, low, high):
+    return max(low, min(high, int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["append", "fp8", "select", "sparse"])
+    hq, hkv, dim = rng.choice(GEOMETRIES)
+    case = {"kind": kind, "hq": hq, "hkv": hkv, "dim": dim}
+    if kind == "append":
+        case["cache"] = rng.choice(["bf16", "e4m3"])
+        case["half"] = rng.choice([dim // 2, dim // 4, dim // 8])
+        case["interleaved"] = rng.choice([False, False, True])
+        if rng.random() < 0.5:
+            case.update(batch=_log(rng, 1, 256), low=1, high=1)
+            case["padded"] = rng.choice([0, rng.randint(0, case["batch"] - 1)])
+        else:
+            case["batch"] = _log(rng, 1, 8)
+            case["high"] = _log(rng, 1, 8192 // case["batch"])
+            case.update(low=rng.randint(1, case["high"]), padded=0)
+        return case
+    case["batch"] = _log(rng, 1, 128)
+    token = hkv * dim * (1 if kind == "fp8" else 2)
+    case["high"] = _log(rng, 1024 if kind == "select" else 16,
+                        min(131072, int(2e9) // (case["batch"] * token)))
+    case["low"] = rng.choice([1, case["high"]])
+    if kind != "fp8":
+        case["kept"] = _log(rng, 4, 128)
+    if kind == "select":                  # at least one sequence has a choice
+        case["kept"] = min(case["kept"], case["high"] // (2 * BLOCK))
+    if kind == "sparse":
+        case["cache"] = rng.choice(["bf16", "e4m3"])
+    return case
+
+
+def _generator(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _normal(gen, *shape):
+    return torch.randn(shape, generator=gen, device=DEV, dtype=torch.bfloat16)
+
+
+def _uniform(gen, low, high, *shape):
+    return torch.rand(shape, generator=gen, device=DEV) * (high - low) + low
+
+
+def _lengths(case):
+    """Tokens per sequence in [low, high], one of them high itself; the same for every seed,
+    so that outputs keep their shapes."""
+    rng = np.random.default_rng([case["low"], case["high"], case["batch"]])
+    lens = rng.integers(case["low"], case["high"] + 1, case["batch"])
+    lens[rng.integers(case["batch"])] = case["high"]
+    return lens.astype(np.int64)
+
+
+def _tables(lens, seed):
+    """int32 [B, width] on the host, -1 past each sequence's pages, in a random order over the
+    pool, and the number of pages."""
+    counts = -(-lens // PAGE)
+    order = np.random.default_rng([seed, 2]).permutation(int(counts.sum())).astype(np.int32)
+    tables = np.full((len(lens), max(1, int(counts.max()))), -1, np.int32)
+    tables[np.arange(tables.shape[1]) < counts[:, None]] = order
+    return tables, int(counts.sum())
+
+
+def _dev(array):
+    return torch.from_numpy(np.ascontiguousarray(array)).to(DEV)
+
+
+def _append_inputs(case, seed):
+    """Rows of a fused projection, their positions and slots: for a decode step sequences of
+    up to 4096 tokens (the same for every seed), a quarter of them at the end of a block, else
+    whole prompts."""
+    gen, rng = _generator(seed), np.random.default_rng([case["batch"], case["padded"]])
+    hq, hkv, dim, new = case["hq"], case["hkv"], case["dim"], _lengths(case)
+    step = case["high"] == 1
+    start = rng.integers(0, 4096, case["batch"]) if step else np.zeros(case["batch"], np.int64)
+    if step:
+        start[::4] |= BLOCK - 1
+    tables, pages = _tables(start + new, seed)
+    at = np.concatenate([np.arange(a, a + n) for a, n in zip(start, new)])
+    owner = np.repeat(np.arange(case["batch"]), new)
+    slots = tables[owner, at // PAGE].astype(np.int64) * PAGE + at % PAGE
+    slots[len(slots) - case["padded"]:] = -1
+    rows = len(at)
+    kind = TYPES[case["cache"]]
+    inverse = 10000.0 ** (-torch.arange(case["half"], device=DEV, dtype=torch.float64)
+                          / case["half"])
+    angle = torch.arange(8192, device=DEV, dtype=torch.float64)[:, None] * inverse
+    fused = _normal(gen, rows, (hq + 2 * hkv) * dim)
+    q, k, v = (t.view(rows, -1, dim)
+               for t in fused.split([hq * dim, hkv * dim, hkv * dim], 1))
+    scales = [_uniform(gen, 0.005, 0.02, hkv) if case["cache"] == "e4m3" else None
+              for _ in range(2)]
+    return dict(q=q, k=k, v=v, positions=_dev(at), slots=_dev(slots.astype(np.int32)),
+                rope=torch.stack([angle.cos(), angle.sin()], -1).float(),
+                k_cache=_normal(gen, pages, PAGE, hkv, dim).to(kind),
+                v_cache=_normal(gen, pages, PAGE, hkv, dim).to(kind),
+                bounds=torch.zeros((pages, PAGE // BLOCK, hkv, 2, dim), device=DEV,
+                                   dtype=torch.bfloat16),
+                k_scale=scales[0], v_scale=scales[1])
+
+
+def _kept_blocks(case, lens, seed):
+    """int32 [B, Hkv, kept]: the first and the last block and a random choice between them,
+    ascending, -1 behind a short sequence's."""
+    rng = np.random.default_rng([seed, 5])
+    out = np.full((case["batch"], case["hkv"], case["kept"]), -1, np.int32)
+    for b, n in enumerate(-(-lens // BLOCK)):
+        for g in range(case["hkv"]):
+            if n <= case["kept"]:
+                out[b, g, :n] = np.arange(n)
+            else:
+                mid = 1 + rng.permutation(n - 2)[:case["kept"] - 2]
+                out[b, g] = np.sort(np.concatenate([[0, n - 1], mid]))
+    return out
+
+
+def _decode_inputs(case, seed):
+    gen = _generator(seed)
+    hq, hkv, dim = case["hq"], case["hkv"], case["dim"]
+    lens = _lengths(case)
+    tables, pages = _tables(lens, seed)
+    x = dict(lens=lens, tables=_dev(tables), lengths=_dev(lens.astype(np.int32)),
+             q=_normal(gen, case["batch"], hq, dim), k_scale=None, v_scale=None)
+    if case["kind"] == "select":
+        # bounds around a mean that drifts from block to block, as keys of a text's parts do
+        middle = _normal(gen, pages, PAGE // BLOCK, hkv, 1, dim) * 0.5
+        spread = _normal(gen, pages, PAGE // BLOCK, hkv, 2, dim).abs() * 0.5 + 1.5
+        spread[..., 0, :].neg_()
+        x["bounds"] = middle + spread
+        return x
+    kind = E4M3 if case["kind"] == "fp8" else TYPES[case["cache"]]
+    x["k"], x["v"] = (_normal(gen, pages, PAGE, hkv, dim).to(kind) for _ in range(2))
+    if kind == E4M3:
+        x["k_scale"], x["v_scale"] = (_uniform(gen, 0.5, 1.5, hkv) for _ in range(2))
+    if case["kind"] == "sparse":
+        x["blocks"] = _dev(_kept_blocks(case, lens, seed))
+    return x
+
+
+def _package():
+    """The package's modules of these operators."""
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                        "paged-decode-lab_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from paged_decode import block_decode, kv_append, spec
+    return block_decode, kv_append, spec
+
+
+def prepare(case, seed):
+    if case["kind"] == "append":
+        return dict(case=case, **_append_inputs(case, seed))
+    state = dict(case=case, **_decode_inputs(case, seed))
+    if own:
+        block_decode, _, spec = _package()
+        geometry = spec.DecodeSpec(case["batch"], case["hq"], case["hkv"], case["dim"],
+                                   case["high"])
+        state["resources"] = block_decode.allocate_block_resources(geometry, DEV,
+                                                                   kept=case.get("kept", 0))
+    return state
+
+
+def run(state):
+    case, kind = state["case"], state["case"]["kind"]
+    if not own:
+        return {"append": _plain_append, "fp8": _plain_fp8, "select": _plain_select,
+                "sparse": _plain_sparse}[kind](state)
+    block_decode, kv_append, _ = _package()
+    if kind == "append":
+        q = kv_append.append_kv(state["q"], state["k"], state["v"], state["positions"],
+                                state["rope"], state["k_cache"], state["v_cache"],
+                                state["slots"], interleaved=case["interleaved"],
+                                k_scale=state["k_scale"], v_scale=state["v_scale"],
+                                bounds=state["bounds"])
+        return {"q": q, "k_cache": state["k_cache"], "v_cache": state["v_cache"],
+                "bounds": state["bounds"]}
+    if kind == "fp8":
+        return block_decode.fp8_decode(state["q"], state["k"], state["v"], state["tables"],
+                                       state["lengths"], resources=state["resources"],
+                                       k_scale=state["k_scale"], v_scale=state["v_scale"])
+    if kind == "select":
+        return block_decode.select_blocks(state["q"], state["bounds"], state["tables"],
+                                          state["lengths"], resources=state["resources"])
+    return block_decode.sparse_decode(state["q"], state["k"], state["v"], state["tables"],
+                                      state["lengths"], state["blocks"],
+                                      resources=state["resources"], k_scale=state["k_scale"],
+                                      v_scale=state["v_scale"])
+
+
+# ------------------------------------------------------------------ plain forms
+
+def _rotated(x, cos, sin, interleaved):
+    half = cos.shape[-1]
+    turned = x[..., :2 * half]
+    if interleaved:
+        a, b = turned[..., 0::2], turned[..., 1::2]
+        turned = torch.stack([a * cos - b * sin, b * cos + a * sin], -1).flatten(-2)
+    else:
+        a, b = turned[..., :half], turned[..., half:]
+        turned = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+    return torch.cat([turned, x[..., 2 * half:]], -1)
+
+
+def _plain_append(s):
+    case = s["case"]
+    hkv, dim, kind = case["hkv"], case["dim"], TYPES[case["cache"]]
+    cos, sin = s["rope"][s["positions"]].unsqueeze(1).unbind(-1)
+    q = _rotated(s["q"].float(), cos, sin, case["interleaved"]).to(torch.bfloat16)
+    new = (_rotated(s["k"].float(), cos, sin, case["interleaved"]), s["v"].float())
+    live = s["slots"] >= 0
+    slots = s["slots"][live].long()
+    for x, cache, scale in zip(new, (s["k_cache"], s["v_cache"]), (s["k_scale"], s["v_scale"])):
+        if scale is not None:
+            x = (x / scale[:, None]).clamp(-E4M3_MAX, E4M3_MAX)
+        bits = torch.uint8 if kind == E4M3 else torch.int16
+        cache.view(bits).view(-1, hkv, dim)[slots] = x[live].to(kind).view(bits)
+    full = slots[slots % BLOCK == BLOCK - 1] // BLOCK
+    keys = s["k_cache"].view(torch.uint8).view(-1, BLOCK, hkv, dim * kind.itemsize)[full]
+    keys = keys.view(kind).float()
+    s["bounds"].view(-1, hkv, 2, dim)[full] = torch.stack([keys.amin(1), keys.amax(1)],
+                                                          2).to(torch.bfloat16)
+    return {"q": q, "k_cache": s["k_cache"], "v_cache": s["v_cache"], "bounds": s["bounds"]}
+
+
+def _gathered(cache, slots):
+    """float32 [..., Hkv, D] of the cache's rows `slots`."""
+    rows = cache.view(torch.uint8).view(-1, cache.shape[2], cache.shape[3] * cache.itemsize)
+    return rows[slots].view(cache.dtype).float()
+
+
+def _attended(q, keys, values, seen, k_scale, v_scale):
+    """q [B, Hkv, G, D], keys and values [B, Hkv, T, D], seen [B, Hkv or 1, T]."""
+    b, hkv, group, dim = q.shape
+    scores = torch.matmul(q.float(), keys.transpose(2, 3).contiguous()) * dim ** -0.5
+    if k_scale is not None:
+        scores *= k_scale[:, None, None]
+    scores.masked_fill_(~seen[:, :, None], float("-inf"))
+    top = scores.amax(-1, keepdim=True)
+    weights = torch.exp(scores - torch.where(top == float("-inf"), 0.0, top))
+    total = weights.sum(-1, keepdim=True)
+    out = torch.matmul(weights, values) / torch.where(total == 0, 1.0, total)
+    if v_scale is not None:
+        out *= v_scale[:, None, None]
+    return out.view(b, hkv * group, dim).to(torch.bfloat16)
+
+
+def _plain_fp8(s):
+    case = s["case"]
+    at = torch.arange(s["tables"].shape[1] * PAGE, device=DEV)[:case["high"]]
+    slots = s["tables"].long().clamp(min=0)[:, at // PAGE] * PAGE + at % PAGE
+    seen = (at < s["lengths"][:, None])[:, None]
+    keys, values = (_gathered(s[n], slots).transpose(1, 2).contiguous() for n in ("k", "v"))
+    q = s["q"].view(case["batch"], case["hkv"], -1, case["dim"])
+    return _attended(q, keys, values, seen, s["k_scale"], s["v_scale"])
+
+
+def _plain_select(s, first=1, last=1):
+    case = s["case"]
+    batch, hkv, dim, kept = case["batch"], case["hkv"], case["dim"], case["kept"]
+    many = s["tables"].shape[1] * (PAGE // BLOCK)
+    j = torch.arange(many, device=DEV)
+    at = s["tables"].long().clamp(min=0).repeat_interleave(PAGE // BLOCK, 1)
+    bounds = s["bounds"].view(-1, PAGE // BLOCK, hkv, 2, dim)[at, j % (PAGE // BLOCK)]
+    bounds = bounds.permute(0, 2, 3, 4, 1).double().contiguous()       # [B, Hkv, 2, D, blocks]
+    q = s["q"].view(batch, hkv, -1, dim).double()
+    scores = (torch.matmul(q.clamp(max=0), bounds[:, :, 0])
+              + torch.matmul(q.clamp(min=0), bounds[:, :, 1])).amax(2)
+    count = -(-s["lengths"].long() // BLOCK)[:, None, None]
+    forced = (j < first) | (j >= count - last)
+    scores = torch.where(forced, float("inf"), scores)
+    scores = torch.where(j < count, scores, float("-inf"))
+    order = torch.sort(scores, dim=-1, descending=True, stable=True).indices[..., :kept]
+    order = torch.where(order < count, order, many).sort(-1).values
+    order = torch.nn.functional.pad(order, (0, kept - order.shape[-1]), value=many)
+    return torch.where(order < many, order, -1).to(torch.int32)
+
+
+def _plain_sparse(s):
+    case = s["case"]
+    batch, hkv, dim = case["batch"], case["hkv"], case["dim"]
+    token = (s["blocks"].long()[..., None] * BLOCK
+             + torch.arange(BLOCK, device=DEV)).flatten(2)             # [B, Hkv, T]
+    seen = (token >= 0) & (token < s["lengths"][:, None, None])
+    token = torch.where(seen, token, 0)
+    owner = torch.arange(batch, device=DEV)[:, None, None]
+    slots = s["tables"].long().clamp(min=0)[owner, token // PAGE] * PAGE + token % PAGE
+    head = torch.arange(hkv, device=DEV)[None, :, None]
+    keys, values = (
+        s[n].view(torch.uint8).view(-1, hkv, dim * s[n].itemsize)[slots, head].view(s[n].dtype)
+        .float() for n in ("k", "v"))
+    q = s["q"].view(batch, hkv, -1, dim)
+    return _attended(q, keys, values, seen, s["k_scale"], s["v_scale"])
+
+
+# ------------------------------------------------------------------ what a pass needs
+
+def work(case):
+    hq, hkv, dim, lens = case["hq"], case["hkv"], case["dim"], _lengths(case)
+    batch, row = case["batch"], case["hkv"] * case["dim"]
+    if case["kind"] == "append":
+        rows, size = int(lens.sum()), TYPES[case["cache"]].itemsize
+        live = rows - case["padded"]
+        turns = rows if case["high"] == 1 else case["high"]     # prompts share their positions
+        return {"bytes": rows * (4 * hq * dim + 4 * row + 12) + turns * 8 * case["half"]
+                + live * 2 * row * size,
+                "flops": 6 * rows * (hq + hkv) * case["half"]}
+    entries = int((-(-lens // PAGE)).sum())
+    small = batch * (2 * hq * dim + 4) + 4 * entries
+    if case["kind"] == "select":
+        # the forced first and last blocks need no score, nor does any of a short sequence
+        counts = -(-lens // BLOCK)
+        scored = int(np.where(counts > case["kept"], counts - 2, 0).sum())
+        return {"bytes": small + scored * hkv * 4 * dim + 4 * batch * hkv * case["kept"],
+                "flops": 2 * scored * hq * dim}
+    if case["kind"] == "fp8":
+        seen, size = int(lens.sum()), 1
+    else:
+        counts = -(-lens // BLOCK)
+        size = TYPES[case["cache"]].itemsize
+        seen = int(np.where(counts > case["kept"],
+                            case["kept"] * BLOCK - (counts * BLOCK - lens), lens).sum())
+        small += 4 * batch * hkv * case["kept"]
+    return {"bytes": small + batch * 2 * hq * dim + seen * 2 * row * size,
+            "flops": 4 * seen * hq * dim}
+
+
+# ------------------------------------------------------------------ in 64 bits
+
+def _exact_rotation(x, positions, rope, interleaved):
+    out, half = x.double().clone(), rope.shape[1]
+    cos, sin = rope[positions].double()[:, None].unbind(-1)
+    first = slice(0, 2 * half, 2) if interleaved else slice(0, half)
+    second = slice(1, 2 * half, 2) if interleaved else slice(half, 2 * half)
+    a, b = out[..., first].clone(), out[..., second].clone()
+    out[..., first], out[..., second] = cos * a - sin * b, sin * a + cos * b
+    return out
+
+
+def _exact_append(case, x):
+    turn = lambda t: _exact_rotation(t, x["positions"], x["rope"], case["interleaved"])  # noqa: E731
+    slots = x["slots"].long().tolist()
+    live = torch.tensor([i for i, s in enumerate(slots) if s >= 0], device=DEV, dtype=torch.long)
+    places = x["slots"].long()[live]
+    found = {"q": turn(x["q"])}
+    for name, rows in (("k", turn(x["k"])), ("v", x["v"].double())):
+        cache = x[name + "_cache"].double()
+        if x[name + "_scale"] is not None:
+            rows = (rows / x[name + "_scale"].double()[:, None]).clamp(-E4M3_MAX, E4M3_MAX)
+        cache.view(-1, case["hkv"], case["dim"])[places] = rows[live]
+        found[name + "_cache"] = cache
+    stored = found["k_cache"]
+    if case["cache"] == "e4m3":       # bounds of the keys as they are stored, no rounding of its own
+        stored = stored.to(E4M3).double()
+    bounds = x["bounds"].double()
+    ends = torch.tensor([s // BLOCK for s in slots if s >= 0 and s % BLOCK == BLOCK - 1],
+                        device=DEV, dtype=torch.long)
+    if len(ends):
+        keys = stored.view(-1, BLOCK, case["hkv"], case["dim"])[ends]
+        bounds.view(-1, case["hkv"], 2, case["dim"])[ends] = torch.stack(
+            [keys.min(1).values, keys.max(1).values], 2)
+    found["bounds"] = bounds
+    return found
+
+
+def _exact_rows(q, keys, values, scale, v_scale):
+    """One kv head: q [G, D], keys and values [T, D] in 64 bits."""
+    weights = torch.softmax((keys @ q.T) * scale, 0)
+    return (weights.T @ values) * v_scale
+
+
+def _slot_rows(cache, table, tokens, head):
+    return cache[table[tokens // PAGE].long(), tokens % PAGE, head]
+
+
+def exact(case, seed):
+    if case["kind"] == "append":
+        return _exact_append(case, _append_inputs(case, seed))
+    x = _decode_inputs(case, seed)
+    hkv, dim = case["hkv"], case["dim"]
+    group = case["hq"] // hkv
+    q = x["q"].double().view(case["batch"], hkv, group, dim)
+    if case["kind"] == "select":
+        return _exact_select(case, x, q)
+    out = torch.zeros(q.shape, device=DEV, dtype=torch.float64)
+    whole = {n: x[n] for n in ("k", "v")}
+    if whole["k"].dtype == E4M3:
+        whole = {n: t.view(torch.uint8) for n, t in whole.items()}
+    as_values = lambda t: (t.view(E4M3) if t.dtype == torch.uint8 else t).double()  # noqa: E731
+    for b, n in enumerate(x["lens"]):
+        for g in range(hkv):
+            tokens = torch.arange(int(n), device=DEV)
+            if case["kind"] == "sparse":
+                listed_ones = x["blocks"][b, g].long()
+                listed_ones = listed_ones[listed_ones >= 0]
+                tokens = (listed_ones[:, None] * BLOCK + torch.arange(BLOCK, device=DEV)).flatten()
+                tokens = tokens[tokens < int(n)]
+            keys, values = (as_values(_slot_rows(whole[c], x["tables"][b], tokens, g).contiguous())
+                            for c in ("k", "v"))
+            if len(tokens):
+                scales = [1.0 if x[c] is None else x[c][g].double() for c in ("k_scale", "v_scale")]
+                out[b, g] = _exact_rows(q[b, g], keys, values, dim ** -0.5 * scales[0], scales[1])
+    return out.view(case["batch"], hkv * group, dim)
+
+
+def _exact_select(case, x, q, first=1, last=1):
+    kept, per = case["kept"], PAGE // BLOCK
+    out = np.full((case["batch"], case["hkv"], kept), -1, np.int32)
+    for b, n in enumerate(-(-x["lens"] // BLOCK)):
+        if n <= kept:
+            out[b, :, :n] = np.arange(n)
+            continue
+        j = torch.arange(first, int(n) - last, device=DEV)
+        bounds = x["bounds"][x["tables"][b, j // per].long(), j % per].double()
+        for g in range(case["hkv"]):
+            part = bounds[:, g, :, None] * q[b, g]                       # [blocks, 2, G, D]
+            scores = part.amax(1).sum(-1).amax(-1).cpu().numpy()
+            best = np.lexsort((np.arange(len(scores)), -scores))[:kept - first - last]
+            out[b, g] = np.concatenate([np.arange(first), np.sort(best) + first,
+                                        np.arange(n - last, n)])
+    return torch.from_numpy(out).to(DEV)
