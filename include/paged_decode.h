@@ -437,6 +437,73 @@ int pd_delta_step(const float* act, const void* a, const void* b, const void* a_
                   void* out, int32_t batch, int32_t hk, int32_t hv, int32_t dk, int32_t dv,
                   int32_t has_prev, pd_stream_t stream);
 
+/* Cache operators of a serving step: keys and values into a bf16 or e4m3 cache
+ * with the position rotation on the way, attention over an e4m3 cache, and
+ * attention over the blocks of a cache that a bound of their keys selects.  No
+ * counterpart in the reference.  Caches are NHD as above, [slots, Hkv, D]. */
+
+#define PD_BLOCK 64 /* tokens per block, four blocks a page */
+#define PD_CACHE_BF16 0
+#define PD_CACHE_E4M3 1 /* float8 e4m3fn; stored value x scale[kv head] (float32, null: 1) */
+
+/* Row i: the leading 2 half elements of its query and key heads rotated by
+ * rope[positions[i]] (float32 [max_positions, half, 2]: cos, sin), pairs (j, j +
+ * half) or, interleaved, (2j, 2j + 1); half 0: no rotation, positions and rope
+ * may be null.  q [rows, Hq, D] -> q_out (may be q); key and value -> slot
+ * slot_mapping[i] of the caches, in an e4m3 cache as round(clamp(x / scale,
+ * +-448)).  A slot outside [0, num_slots) skips the write; a position outside
+ * the table too, and the rotated part of its query is NaN.  Slots of one call
+ * must differ.  Row strides are in elements, multiples of 8, heads contiguous;
+ * half is a multiple of 8; num_heads may be 0.  bounds (may be null): as
+ * pd_block_bounds, of the keys just written. */
+int pd_append_kv(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                 int64_t v_stride, const int64_t* positions, const float* rope,
+                 int64_t max_positions, int32_t half, int32_t interleaved, void* q_out,
+                 int64_t q_out_stride, void* k_cache, void* v_cache, int32_t cache_type,
+                 int64_t num_slots, const int32_t* slot_mapping, const float* k_scale,
+                 const float* v_scale, void* bounds, int64_t rows, int32_t num_heads,
+                 int32_t num_kv_heads, int32_t head_dim, pd_stream_t stream);
+
+/* bounds bf16 [num_slots / 64, Hkv, 2, D]: smallest and largest stored key of
+ * every block whose last slot (slot % 64 == 63) is in slot_mapping [rows]. */
+int pd_block_bounds(const void* k_cache, int32_t cache_type, int64_t num_slots,
+                    const int32_t* slot_mapping, int64_t rows, void* bounds, int32_t num_kv_heads,
+                    int32_t head_dim, pd_stream_t stream);
+
+/* blocks int32 [batch, Hkv, kept]: of a sequence's ceil(length / 64) blocks the
+ * first `first` and last `last` (at least 1: a block that is not full has no
+ * bounds) and those of the highest scores, score = max over the group's query
+ * heads of sum_d max(q, 0) high + min(q, 0) low in 64 bits, ties to the lowest
+ * block; ascending, -1 behind a sequence of fewer.  A NaN score counts as
+ * +infinity, a page outside [0, num_pages) as the lowest.  keys: workspace uint64
+ * [batch, Hkv, table_width * 4]. */
+int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* bounds,
+                     int64_t num_pages, const int32_t* table, int64_t table_stride_b,
+                     int32_t table_width, const int32_t* lengths, uint64_t* keys, int32_t* blocks,
+                     int32_t kept, int32_t first, int32_t last, int32_t batch, int32_t num_heads,
+                     int32_t num_kv_heads, int32_t head_dim, pd_stream_t stream);
+
+/* Splits of pd_block_decode for a batch whose rows have up to `entries` blocks:
+ * it depends on the batch through its next power of two alone.  Host only. */
+#define PD_BLOCK_SPLITS 128
+int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t entries,
+                    int32_t cus, int32_t* splits);
+
+/* out bf16 [batch, Hq, D] = softmax(scale k_scale q K^T) V v_scale over the tokens
+ * below the length of the blocks listed for the sequence and kv head (int32
+ * [batch, Hkv, kept]; null: of every block).  Entries below 0 or past the length
+ * and pages outside [0, num_pages) have no tokens, an entry that is listed twice
+ * counts twice, a row without tokens is 0.  With splits > 1 the blocks are cut
+ * into that many spans (part_o float32 [batch, Hq, splits, D], part_ml [batch,
+ * Hq, splits, 2]) and a second launch joins them. */
+int pd_block_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k,
+                    const void* v, int32_t cache_type, int64_t num_pages, const int32_t* table,
+                    int64_t table_stride_b, int32_t table_width, const int32_t* lengths,
+                    const int32_t* blocks, int32_t kept, const float* k_scale,
+                    const float* v_scale, float* part_o, float* part_ml, int32_t splits, void* out,
+                    int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                    double scale, pd_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,168 @@
+"""Decode attention over an e4m3 cache, and over the blocks of a cache that matter.
+
+``fp8_decode``     one query token per sequence over its whole e4m3 cache
+                   (``kv_append.append_kv`` writes it), half the bytes of a bf16 one;
+``select_blocks``  per sequence and kv head the blocks of 64 tokens whose keys can score
+                   highest for the group's queries, by the bounds that append_kv keeps;
+``sparse_decode``  one query token per sequence over the listed blocks, bf16 or e4m3.
+
+Contract as of ``runtime.paged_decode``: outputs and workspaces belong to the resources and
+are overwritten by the next call with them, two streams may not use them at once, contents
+are not checked, nothing allocates, synchronizes or reads device memory on the host (a step
+can be captured in a hipGraph).  Lengths past the table count as its capacity; a page outside
+the cache is read as having no tokens.  A sequence's output depends on the batch through its
+next power of two alone, so a padded graph bucket gives the bits of the eager call.
+"""
+from dataclasses import dataclass, field
+import math
+
+import torch
+
+from . import _native
+from .kv_append import check_scales
+from .runtime import _device_cus
+
+BLOCK = _native.BLOCK
+_PER_PAGE = 256 // BLOCK
+E4M3 = torch.float8_e4m3fn
+
+
+@dataclass
+class BlockResources:
+    spec: object
+    kept: int                       # blocks listed per sequence and kv head, 0: every block
+    out: torch.Tensor
+    partials: torch.Tensor          # float32, flat: [B, Hq, splits, D] of a call
+    sums: torch.Tensor              # float32, flat: [B, Hq, splits, 2]
+    blocks: torch.Tensor | None = None
+    keys: torch.Tensor | None = None
+    sm_count: int = 0
+    _splits: dict = field(default_factory=dict, repr=False, compare=False)
+
+    def splits(self, batch):
+        found = self._splits.get(batch)
+        if found is None:
+            spec = self.spec
+            found = self._splits[batch] = _native.block_splits(
+                batch, spec.num_heads, spec.num_kv_heads,
+                self.kept or spec.table_width * _PER_PAGE, self.sm_count)
+        return found
+
+
+def allocate_block_resources(spec, device, *, kept=0):
+    """Output and workspace of ``fp8_decode`` (kept 0), or of ``select_blocks`` and
+    ``sparse_decode`` with ``kept`` blocks of 64 tokens per sequence and kv head."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError("block resources require CUDA")
+    if type(kept) is not int or kept < 0:
+        raise ValueError("kept must be a non-negative integer")
+    make = lambda *shape, dtype=torch.float32: torch.empty(shape, device=device, dtype=dtype)  # noqa: E731
+    heads, hkv, dim = spec.num_heads, spec.num_kv_heads, spec.head_dim
+    out = make(spec.max_batch, heads, dim, dtype=torch.bfloat16)
+    result = BlockResources(spec, kept, out, out, out, sm_count=_device_cus(device))
+    rows, batch = 0, 1
+    while batch < 2 * spec.max_batch:
+        batch = min(batch, spec.max_batch)
+        splits = result.splits(batch)
+        rows = max(rows, batch * heads * splits if splits > 1 else 0)
+        batch *= 2
+    result.partials, result.sums = make(rows * dim), make(rows * 2)
+    if kept:
+        result.blocks = make(spec.max_batch, hkv, kept, dtype=torch.int32)
+        result.keys = make(spec.max_batch, hkv, spec.table_width * _PER_PAGE, dtype=torch.int64)
+    return result
+
+
+def _check_step(q, tables, lengths, resources):
+    spec = resources.spec
+    device = q.get_device()
+    if device < 0 or not (tables.get_device() == lengths.get_device()
+                          == resources.out.get_device() == device):
+        raise ValueError("all tensors must be on the same CUDA device")
+    if q.dtype != torch.bfloat16:
+        raise ValueError("BF16 Q required")
+    if q.ndim != 3 or q.shape[1:] != (spec.num_heads, spec.head_dim):
+        raise ValueError("Q must have shape [batch, query_heads, head_dim]")
+    batch = q.shape[0]
+    if not 0 < batch <= spec.max_batch or q.stride(2) != 1:
+        raise ValueError("Q batch exceeds capacity or innermost dimension is not contiguous")
+    if tables.ndim != 2 or tables.shape[0] != batch or tables.stride(1) != 1:
+        raise ValueError("block table must have shape [batch,capacity] and contiguous rows")
+    if not 0 < tables.shape[1] <= spec.table_width:
+        raise ValueError("block table width outside configured capacity")
+    if lengths.shape != (batch,) or not lengths.is_contiguous():
+        raise ValueError("context lengths must be a contiguous [batch] tensor")
+    if tables.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise ValueError("block tables and context lengths must be int32")
+    return batch, device
+
+
+def _attend(q, k, v, tables, lengths, blocks, resources, scale, k_scale, v_scale):
+    batch, device = _check_step(q, tables, lengths, resources)
+    spec = resources.spec
+    if k.dtype not in _native.CACHE_TYPES or v.dtype != k.dtype:
+        raise ValueError("caches must be BF16 or float8_e4m3fn")
+    if k.ndim != 4 or k.shape[1:] != (256, spec.num_kv_heads, spec.head_dim):
+        raise ValueError("KV must use NHD pages [pages,256,kv_heads,head_dim]")
+    if k.shape != v.shape or not k.is_contiguous() or not v.is_contiguous() or k.shape[0] == 0:
+        raise ValueError("K/V must have matching nonempty contiguous storage")
+    if k.get_device() != device or v.get_device() != device:
+        raise ValueError("all tensors must be on the same CUDA device")
+    check_scales(k_scale, v_scale, k.dtype, spec.num_kv_heads, device)
+    scale = spec.head_dim ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    splits = resources.splits(batch)
+    _native.block_decode(q, k, v, tables, lengths, blocks, k_scale, v_scale, resources.partials,
+                         resources.sums, splits, resources.out, spec.num_kv_heads, scale)
+    return resources.out if batch == spec.max_batch else resources.out[:batch]
+
+
+def fp8_decode(q, k, v, tables, lengths, *, resources, scale=None, k_scale=None, v_scale=None):
+    """Attention of q [B, Hq, D] bf16 over e4m3 pages k, v [pages, 256, Hkv, D], whose values
+    are the stored ones times ``k_scale`` and ``v_scale`` (float32 [Hkv], None: 1); returns
+    ``resources.out[:B]``.  An empty sequence gives zeros."""
+    if k.dtype != E4M3:
+        raise ValueError("fp8_decode reads a float8_e4m3fn cache; paged_decode reads a BF16 one")
+    if resources.kept:
+        raise ValueError("these resources are sized for a list of blocks")
+    return _attend(q, k, v, tables, lengths, None, resources, scale, k_scale, v_scale)
+
+
+def select_blocks(q, bounds, tables, lengths, *, resources, first=1, last=1):
+    """int32 [B, Hkv, kept]: the blocks that ``sparse_decode`` should read, ascending, -1 behind
+    a sequence of fewer.
+
+    Of a sequence's ceil(length / 64) blocks the first ``first`` and last ``last`` are always
+    in; the others by score, the largest of the group's query heads' sums over the channels of
+    max(q, 0) high + min(q, 0) low, computed in 64 bits; ties go to the lowest block.
+    ``bounds`` as of ``kv_append``, of the keys as they are stored (a scale per kv head moves
+    no block).  ``last`` is at least 1: the block being filled has no bounds.  A NaN score
+    counts as infinite."""
+    batch, device = _check_step(q, tables, lengths, resources)
+    spec = resources.spec
+    if not resources.kept:
+        raise ValueError("these resources hold no list of blocks: allocate them with kept=")
+    if (bounds.shape[1:] != (_PER_PAGE, spec.num_kv_heads, 2, spec.head_dim)
+            or bounds.dtype != torch.bfloat16 or not bounds.is_contiguous()
+            or bounds.get_device() != device or bounds.shape[0] == 0):
+        raise ValueError("bounds must be contiguous BF16 [pages, 4, kv_heads, 2, head_dim]")
+    _native.select_blocks(q, bounds, tables, lengths, resources.keys, resources.blocks,
+                          spec.num_kv_heads, first, last)
+    return resources.blocks if batch == spec.max_batch else resources.blocks[:batch]
+
+
+def sparse_decode(q, k, v, tables, lengths, blocks, *, resources, scale=None, k_scale=None,
+                  v_scale=None):
+    """Attention of q [B, Hq, D] bf16 over the tokens below the length of the listed blocks,
+    int32 [B, Hkv, listed <= kept] (``select_blocks``, or any choice); pages bf16 or
+    float8_e4m3fn as in ``fp8_decode``; returns ``resources.out[:B]``.  Entries below 0 or past
+    the length have no tokens, an entry listed twice counts twice, no token gives zeros."""
+    if not resources.kept:
+        raise ValueError("these resources hold no list of blocks: allocate them with kept=")
+    if (blocks.ndim != 3 or blocks.shape[:2] != (q.shape[0], resources.spec.num_kv_heads)
+            or not 0 < blocks.shape[2] <= resources.kept or blocks.dtype != torch.int32
+            or not blocks.is_contiguous() or blocks.get_device() != q.get_device()):
+        raise ValueError("blocks must be contiguous int32 [batch, kv_heads, listed], at most kept")
+    return _attend(q, k, v, tables, lengths, blocks, resources, scale, k_scale, v_scale)
