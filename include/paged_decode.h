@@ -483,11 +483,13 @@ int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_stride_h, cons
                      int32_t kept, int32_t first, int32_t last, int32_t batch, int32_t num_heads,
                      int32_t num_kv_heads, int32_t head_dim, pd_stream_t stream);
 
-/* Splits of pd_block_decode for a batch whose rows have up to `entries` blocks:
- * it depends on the batch through its next power of two alone.  Host only. */
+/* Splits of pd_block_decode for a batch whose rows have up to `entries` blocks,
+ * listed or the whole cache's: they depend on the batch through its next power of
+ * two alone.  Host only. */
 #define PD_BLOCK_SPLITS 128
-int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t entries,
-                    int32_t cus, int32_t* splits);
+int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                    int32_t cache_type, int32_t entries, int32_t listed, int32_t cus,
+                    int32_t* splits);
 
 /* out bf16 [batch, Hq, D] = softmax(scale k_scale q K^T) V v_scale over the tokens
  * below the length of the blocks listed for the sequence and kv head (int32

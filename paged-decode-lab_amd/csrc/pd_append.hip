@@ -12,6 +12,14 @@
 //
 // Bound: HBM bytes.  A thread takes 16 elements of a head, for a rotated head
 // both halves of eight pairs, so nothing crosses a lane.
+//
+// Bounds (smallest and largest stored key per channel) are made of the blocks of
+// 64 slots whose last slot a call writes: for prompts in a second launch, from the
+// cache.  A decode step's rows have them made in the launch that writes them.
+// A block's other keys may be written by other workgroups of it, so the one that
+// makes the bounds takes this call's keys from their source, rotated and rounded
+// as they are stored, and the others from the cache; no workgroup waits for
+// another.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -31,16 +39,27 @@ using pd::u16;
 
 struct AppendArgs {
   const uint16_t *q, *k, *v;
-  const int64_t* positions;
   const float* rope;
   uint16_t* q_out;
   char *k_cache, *v_cache;
-  const int32_t* slots;
   const float *k_scale, *v_scale;
-  int64_t q_stride, k_stride, v_stride, q_out_stride, max_positions, num_slots;
-  uint32_t rows, items_per_row;
+  uint16_t* bounds;  // or null
+  int64_t q_stride, k_stride, v_stride, q_out_stride, max_positions;
   int hq, hkv, half;
 };
+
+// x / d for a positive normal d whose reciprocal `inverse` is correctly rounded: two
+// corrections by the remainder, which an FMA gives exactly, leave the correctly rounded
+// quotient (the first is within an ulp, the second has the exact remainder of it); five
+// operations, a division is ten.  A quotient that is clamped or becomes a zero (whose sign the
+// corrections would lose), an infinity or a NaN stays as it is.
+__device__ __forceinline__ float divide(float x, float d, float inverse) {
+  const float q = x * inverse;
+  float r = __builtin_fmaf(__builtin_fmaf(-q, d, x), inverse, q);
+  r = __builtin_fmaf(__builtin_fmaf(-r, d, x), inverse, r);
+  const float size = fabsf(q);
+  return size > 1e-6f && size < 1e6f ? r : q;
+}
 
 __device__ __forceinline__ float e4m3_range(float x) {
   const float y = __builtin_amdgcn_fmed3f(x, 448.f, -448.f);
@@ -60,76 +79,235 @@ __device__ __forceinline__ u32x2_t pack8_e4m3(const float (&x)[8]) {
   return r;
 }
 
-// x of eight elements to element `at` of a cache.
-template <bool kE4m3>
-__device__ __forceinline__ void store_cache8(char* cache, int64_t at, float (&x)[8], float scale) {
-  if constexpr (kE4m3) {
+__device__ __forceinline__ void unpack8_e4m3(u32x2_t raw, float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] / scale;
-    *reinterpret_cast<u32x2_t*>(cache + at) = pack8_e4m3(x);
-  } else {
-    *reinterpret_cast<u32x4_t*>(cache + 2 * at) = pack8(x);
+  for (int i = 0; i < 2; ++i) {
+    const floatx2_t a = __builtin_amdgcn_cvt_pk_f32_fp8(raw[i], false);
+    const floatx2_t b = __builtin_amdgcn_cvt_pk_f32_fp8(raw[i], true);
+    x[4 * i] = a[0], x[4 * i + 1] = a[1], x[4 * i + 2] = b[0], x[4 * i + 3] = b[1];
   }
 }
 
-template <int D, bool kE4m3, bool kInterleaved>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
+struct Scale {
+  float value, inverse;
+  __device__ __forceinline__ Scale(const float* scales, int head) {
+    value = scales ? scales[head] : 1.f;
+    inverse = 1.f / value;
+  }
+};
+
+__device__ __forceinline__ u32x2_t to_e4m3(const float (&x)[8], const Scale& scale) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = divide(x[i], scale.value, scale.inverse);
+  return pack8_e4m3(y);
+}
+
+// (x, y) of a pair rotated; each operation rounded by itself.
+__device__ __forceinline__ void rotate(float& x, float& y, float c, float s) {
 #pragma clang fp contract(off)
+  const float u = x * c - y * s, w = y * c + x * s;
+  x = u, y = w;
+}
+
+// (cos, sin) of kPairs pairs from `pair` on.
+template <int kPairs>
+struct Turn {
+  floatx4_t cs[kPairs / 2];
+  __device__ __forceinline__ Turn(const float* rope, int64_t position, int half, int pair) {
+    const floatx4_t* at = reinterpret_cast<const floatx4_t*>(rope + (position * half + pair) * 2);
+#pragma unroll
+    for (int i = 0; i < kPairs / 2; ++i) cs[i] = at[i];
+  }
+  __device__ __forceinline__ float c(int i) const { return cs[i / 2][2 * (i % 2)]; }
+  __device__ __forceinline__ float s(int i) const { return cs[i / 2][2 * (i % 2) + 1]; }
+};
+
+// Channels d..d+7 of row `row`'s key as the cache will hold them (not divided by a scale's
+// effect: the stored value itself).
+template <bool kE4m3, bool kInterleaved>
+__device__ __forceinline__ void stored8(const AppendArgs& p, const int64_t* positions, int64_t row,
+                                        const uint16_t* head, int d, const Scale& scale,
+                                        float (&x)[8]) {
+  unpack8(load16(head + d), x);
+  if (d < 2 * p.half) {
+    const int64_t position = positions[row];
+    if constexpr (kInterleaved) {
+      const Turn<4> turn(p.rope, position, p.half, d / 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rotate(x[2 * i], x[2 * i + 1], turn.c(i), turn.s(i));
+    } else {
+      const bool first = d < p.half;
+      float y[8];
+      unpack8(load16(head + (first ? d + p.half : d - p.half)), y);
+      const Turn<8> turn(p.rope, position, p.half, first ? d : d - p.half);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float a = first ? x[i] : y[i], b = first ? y[i] : x[i];
+        rotate(a, b, turn.c(i), turn.s(i));
+        x[i] = first ? a : b;
+      }
+    }
+  }
+  if constexpr (kE4m3)
+    unpack8_e4m3(to_e4m3(x, scale), x);
+  else
+    unpack8(pack8(x), x);
+}
+
+// Smallest and largest per channel over a workgroup's keys, eight channels of a token a
+// thread; a NaN key leaves a NaN.
+template <int D>
+struct Extremes {
+  static constexpr int kLanes = D / 8;
+  float lo[8], hi[8];
+  __device__ __forceinline__ void add(const float (&x)[8], bool first) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      lo[e] = first ? x[e] : __builtin_elementwise_minimum(lo[e], x[e]);
+      hi[e] = first ? x[e] : __builtin_elementwise_maximum(hi[e], x[e]);
+    }
+  }
+  template <int M>
+  __device__ __forceinline__ void join(int lane) {
+    if constexpr (kLanes <= M) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        lo[e] = __builtin_elementwise_minimum(lo[e], xor_lanes<M>(lo[e], lane));
+        hi[e] = __builtin_elementwise_maximum(hi[e], xor_lanes<M>(hi[e], lane));
+      }
+    }
+  }
+  // Stored values are bf16 or e4m3: bf16 bounds lose no bit.
+  __device__ __forceinline__ void write(float (&low)[4][D], float (&high)[4][D], int tid,
+                                        uint16_t* out) {
+    const int lane = tid & 63, w = tid >> 6;
+    join<32>(lane), join<16>(lane), join<8>(lane);
+    if (lane < kLanes) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) low[w][lane * 8 + e] = lo[e], high[w][lane * 8 + e] = hi[e];
+    }
+    __syncthreads();
+    if (tid < D) {
+      float l = low[0][tid], h = high[0][tid];
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        l = __builtin_elementwise_minimum(l, low[i][tid]);
+        h = __builtin_elementwise_maximum(h, high[i][tid]);
+      }
+      out[tid] = uint16_t(bf16_bits(l));
+      out[D + tid] = uint16_t(bf16_bits(h));
+    }
+    __syncthreads();
+  }
+};
+
+// Bounds of the blocks that end among `per` rows from row0 on, for one kv head; source(t, x)
+// gives false where token t is to be taken from the cache, else this thread's channels of
+// its key.
+template <int D, bool kE4m3, typename Begin, typename Source>
+__device__ __forceinline__ void bounds_of_rows(const int32_t* __restrict__ slots, int64_t rows,
+                                               int64_t num_slots, int64_t row0, int per,
+                                               const char* k_cache, uint16_t* bounds, int hkv,
+                                               int kvh, Begin begin, Source source) {
+  constexpr int kBytes = D * (kE4m3 ? 1 : 2), kLanes = D / 8, kStep = 256 / kLanes;
+  __shared__ float low[4][D], high[4][D];
+  const int tid = threadIdx.x, lane = tid & 63;
+  int32_t slot = lane < per && row0 + lane < rows ? slots[row0 + lane] : -1;
+  if (slot >= num_slots) slot = -1;
+  uint64_t full = __ballot(slot >= 0 && (slot & 63) == 63);
+  while (full) {
+    const int at = __builtin_ctzll(full);
+    const int64_t block = __builtin_amdgcn_readlane(slot, at) >> 6;
+    full &= full - 1;
+    begin(block);
+    const char* base = k_cache + (block * 64 * hkv + kvh) * kBytes + (tid % kLanes) * (kBytes / kLanes);
+    Extremes<D> extremes;
+#pragma unroll 4
+    for (int i = 0; i < 64 / kStep; ++i) {
+      const int t = i * kStep + tid / kLanes;
+      float x[8];
+      if (!source(t, x)) {
+        const char* row = base + int64_t(t) * hkv * kBytes;
+        if constexpr (kE4m3)
+          unpack8_e4m3(*reinterpret_cast<const u32x2_t*>(row), x);
+        else
+          unpack8(*reinterpret_cast<const u32x4_t*>(row), x);
+      }
+      extremes.add(x, i == 0);
+    }
+    extremes.write(low, high, tid, bounds + (block * hkv + kvh) * 2 * D);
+  }
+}
+
+// kBounds: the leading workgroups, one for each row and kv head, make the bounds of the block
+// that the row ends, if it does.  The others: 16 elements of a head a thread.
+template <int D, bool kE4m3, bool kInterleaved, bool kBounds>
+__global__ void __launch_bounds__(256)
+append_kernel(const int32_t* __restrict__ slots, const int64_t* __restrict__ positions,
+              uint32_t rows, uint32_t items_per_row, int64_t num_slots, const AppendArgs p) {
   constexpr int kItems = D / 16;  // of a head
-  const uint32_t id = blockIdx.x * 256 + threadIdx.x;
-  const uint32_t row = id / p.items_per_row;
-  if (row >= p.rows) return;
-  const uint32_t item = id - row * p.items_per_row;
+  const uint32_t bound_groups = kBounds ? rows * p.hkv : 0;
+  if (kBounds && blockIdx.x < bound_groups) {
+    __shared__ int32_t from[64];  // the row that writes a token of the block, or -1
+    const int kvh = int(blockIdx.x % p.hkv), tid = threadIdx.x;
+    const Scale scale(kE4m3 ? p.k_scale : nullptr, kvh);
+    bounds_of_rows<D, kE4m3>(
+        slots, rows, num_slots, blockIdx.x / p.hkv, 1, p.k_cache, p.bounds, p.hkv, kvh,
+        [&](int64_t block) {
+          if (tid < 64) from[tid] = -1;
+          __syncthreads();
+          for (uint32_t i = tid; i < rows; i += 256) {
+            const int32_t slot = slots[i];
+            const int64_t pos = p.half ? positions[i] : 0;
+            if (slot >= 0 && slot >> 6 == block &&
+                (!p.half || (pos >= 0 && pos < p.max_positions)))
+              from[slot & 63] = int32_t(i);
+          }
+          __syncthreads();
+        },
+        [&](int t, float(&x)[8]) {
+          const int64_t r = from[t];
+          if (r < 0) return false;
+          stored8<kE4m3, kInterleaved>(p, positions, r, p.k + r * p.k_stride + kvh * D,
+                                       tid % (D / 8) * 8, scale, x);
+          return true;
+        });
+    return;
+  }
+
+  const uint32_t id = (blockIdx.x - bound_groups) * 256 + threadIdx.x;
+  const uint32_t row = id / items_per_row;
+  if (row >= rows) return;
+  const uint32_t item = id - row * items_per_row;
   const int head = int(item / kItems), t = int(item % kItems);
   const bool query = head < p.hq, value = head >= p.hq + p.hkv;
   const int kvh = query ? 0 : value ? head - p.hq - p.hkv : head - p.hq;
-
-  int64_t slot = 0;
-  if (!query) {
-    slot = p.slots[row];
-    if (slot < 0 || slot >= p.num_slots) return;
-  }
+  const int64_t slot = query ? 0 : slots[row];
+  const int64_t pos = p.half ? positions[row] : 0;
   // The item's two runs of eight elements.
   const int turned = value ? 0 : p.half / 8;
-  int first, second;
-  if (t < turned) {
-    first = kInterleaved ? 16 * t : 8 * t;
-    second = kInterleaved ? first + 8 : first + p.half;
-  } else {
-    first = 16 * t;
-    second = first + 8;
-  }
+  const bool apart = !kInterleaved && t < turned;
+  const int first = apart ? 8 * t : 16 * t, second = apart ? first + p.half : first + 8;
   const uint16_t* src = query   ? p.q + int64_t(row) * p.q_stride + head * D
                         : value ? p.v + int64_t(row) * p.v_stride + kvh * D
                                 : p.k + int64_t(row) * p.k_stride + kvh * D;
   const u32x4_t raw_a = load16(src + first), raw_b = load16(src + second);
+  if (slot < 0 || slot >= num_slots) return;
+  const bool known = !p.half || (pos >= 0 && pos < p.max_positions);
+  if (!known && !query) return;  // no such position: nothing is cached, the query is NaN
   float a[8], b[8];
   unpack8(raw_a, a);
   unpack8(raw_b, b);
   if (t < turned) {
-    const int64_t pos = p.positions[row];
-    if (pos < 0 || pos >= p.max_positions) {
-      if (!query) return;  // no such position: nothing is cached, the query is NaN
+    const Turn<8> turn(p.rope, known ? pos : 0, p.half, 8 * t);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = b[i] = __builtin_nanf("");
-    } else {
-      floatx4_t turn[4];  // (cos, sin) of eight pairs
-      const floatx4_t* table =
-          reinterpret_cast<const floatx4_t*>(p.rope + (pos * p.half + 8 * t) * 2);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) turn[i] = table[i];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float c = turn[i / 2][2 * (i % 2)], s = turn[i / 2][2 * (i % 2) + 1];
-        float& x = kInterleaved ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i];
-        float& y = kInterleaved ? (i < 4 ? a[2 * i + 1] : b[2 * i - 7]) : b[i];
-        const float u = x * c - y * s, w = y * c + x * s;
-        x = u, y = w;
-      }
+    for (int i = 0; i < 8; ++i) {
+      float& x = kInterleaved ? (i < 4 ? a[2 * i] : b[2 * i - 8]) : a[i];
+      float& y = kInterleaved ? (i < 4 ? a[2 * i + 1] : b[2 * i - 7]) : b[i];
+      rotate(x, y, turn.c(i), turn.s(i));
+      if (!known) x = y = __builtin_nanf("");
     }
-  } else if (!query && p.half) {
-    const int64_t pos = p.positions[row];
-    if (pos < 0 || pos >= p.max_positions) return;
   }
   if (query) {
     uint16_t* dst = p.q_out + int64_t(row) * p.q_out_stride + head * D;
@@ -137,98 +315,50 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs p) {
     *reinterpret_cast<u32x4_t*>(dst + second) = pack8(b);
     return;
   }
-  const float* scales = value ? p.v_scale : p.k_scale;
-  const float scale = kE4m3 && scales ? scales[kvh] : 1.f;
   char* cache = value ? p.v_cache : p.k_cache;
   const int64_t at = (slot * p.hkv + kvh) * D;
-  store_cache8<kE4m3>(cache, at + first, a, scale);
-  store_cache8<kE4m3>(cache, at + second, b, scale);
+  if constexpr (kE4m3) {
+    const Scale scale(value ? p.v_scale : p.k_scale, kvh);
+    const u32x2_t x = to_e4m3(a, scale), y = to_e4m3(b, scale);
+    if (second == first + 8) {
+      *reinterpret_cast<u32x4_t*>(cache + at + first) = u32x4_t{x[0], x[1], y[0], y[1]};
+    } else {
+      *reinterpret_cast<u32x2_t*>(cache + at + first) = x;
+      *reinterpret_cast<u32x2_t*>(cache + at + second) = y;
+    }
+  } else {
+    *reinterpret_cast<u32x4_t*>(cache + 2 * (at + first)) = pack8(a);
+    *reinterpret_cast<u32x4_t*>(cache + 2 * (at + second)) = pack8(b);
+  }
 }
 
-// Smallest and largest stored key per channel of the blocks of 64 slots whose
-// last slot is among `slots`.  A workgroup looks at 16 rows for one kv head; a
-// token is kLanes threads of 16 bytes.  A NaN key leaves a NaN.
+// The same from the cache alone.
 template <int D, bool kE4m3>
 __global__ void __launch_bounds__(256)
-block_bounds_kernel(const char* __restrict__ k_cache, const int32_t* __restrict__ slots,
-                    int64_t rows, int64_t num_slots, uint16_t* __restrict__ bounds, int hkv) {
-  constexpr int kBytes = D * (kE4m3 ? 1 : 2), kLanes = kBytes / 16, kStep = 256 / kLanes;
-  constexpr int E = D / kLanes;  // elements of 16 bytes
-  __shared__ float low[4][D], high[4][D];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int64_t row = int64_t(blockIdx.x) * 16 + (lane & 15);
-  const int kvh = blockIdx.y;
-  int32_t slot = row < rows ? slots[row] : -1;
-  if (slot >= num_slots) slot = -1;
-  uint64_t full = __ballot(lane < 16 && slot >= 0 && (slot & 63) == 63);
-  while (full) {
-    const int64_t block = __builtin_amdgcn_readlane(slot, __builtin_ctzll(full)) >> 6;
-    full &= full - 1;
-    const char* base = k_cache + (block * 64 * hkv + kvh) * kBytes + (tid % kLanes) * 16;
-    float lo[E], hi[E];
-    u32x4_t raw[64 / kStep];
-#pragma unroll
-    for (int i = 0; i < 64 / kStep; ++i)
-      raw[i] = *reinterpret_cast<const u32x4_t*>(
-          base + int64_t(i * kStep + tid / kLanes) * hkv * kBytes);
-#pragma unroll
-    for (int i = 0; i < 64 / kStep; ++i)
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        float x, y;
-        if constexpr (kE4m3) {
-          const floatx2_t f = (e & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8(raw[i][e / 4], true)
-                                      : __builtin_amdgcn_cvt_pk_f32_fp8(raw[i][e / 4], false);
-          x = f[0], y = f[1];
-        } else {
-          x = bf16_lo(raw[i][e / 2]), y = bf16_hi(raw[i][e / 2]);
-        }
-        lo[e] = i ? __builtin_elementwise_minimum(lo[e], x) : x;
-        hi[e] = i ? __builtin_elementwise_maximum(hi[e], x) : x;
-        lo[e + 1] = i ? __builtin_elementwise_minimum(lo[e + 1], y) : y;
-        hi[e + 1] = i ? __builtin_elementwise_maximum(hi[e + 1], y) : y;
-      }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-#define PD_JOIN(M)                                                                    \
-  if constexpr (kLanes <= M) {                                                        \
-    lo[e] = __builtin_elementwise_minimum(lo[e], xor_lanes<M>(lo[e], lane));          \
-    hi[e] = __builtin_elementwise_maximum(hi[e], xor_lanes<M>(hi[e], lane));          \
-  }
-      PD_JOIN(32) PD_JOIN(16) PD_JOIN(8) PD_JOIN(4)
-#undef PD_JOIN
-      if (lane < kLanes) {
-        low[w][lane * E + e] = lo[e];
-        high[w][lane * E + e] = hi[e];
-      }
-    }
-    __syncthreads();
-    for (int d = tid; d < D; d += 256) {
-      float l = low[0][d], h = high[0][d];
-#pragma unroll
-      for (int i = 1; i < 4; ++i) {
-        l = __builtin_elementwise_minimum(l, low[i][d]);
-        h = __builtin_elementwise_maximum(h, high[i][d]);
-      }
-      // Stored values are bf16 or e4m3: no bit is lost.
-      uint16_t* out = bounds + (block * hkv + kvh) * 2 * D + d;
-      out[0] = uint16_t(bf16_bits(l));
-      out[D] = uint16_t(bf16_bits(h));
-    }
-    __syncthreads();
-  }
+block_bounds_kernel(const int32_t* __restrict__ slots, const char* __restrict__ k_cache,
+                    uint16_t* __restrict__ bounds, int64_t rows, int64_t num_slots, int per,
+                    int hkv) {
+  bounds_of_rows<D, kE4m3>(slots, rows, num_slots, int64_t(blockIdx.x) * per, per, k_cache, bounds,
+                           hkv, blockIdx.y, [](int64_t) {},
+                           [](int, float(&)[8]) { return false; });
 }
+
+// A decode step has at most this many rows here.  Each may end a block: a workgroup for each
+// row.  Of 64 rows of a prompt one does.
+constexpr int64_t kStepRows = 512;
+int rows_per_group(int64_t rows) { return rows <= kStepRows ? 1 : 64; }
 
 int launch_bounds(const void* k_cache, int32_t cache_type, int64_t num_slots,
                   const int32_t* slot_mapping, int64_t rows, void* bounds, int32_t num_kv_heads,
                   int32_t head_dim, pd_stream_t stream) {
-  const int64_t groups = (rows + 15) / 16;
+  const int per = rows_per_group(rows);
+  const int64_t groups = (rows + per - 1) / per;
   if (groups > 0x7fffffff || num_kv_heads > 65535)
     return pd::fail(PD_EINVAL, "grid dimension exceeds device limits");
   const auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(unsigned(groups), unsigned(num_kv_heads)), dim3(256), 0,
-                       as_stream(stream), static_cast<const char*>(k_cache), slot_mapping, rows,
-                       num_slots, u16(bounds), num_kv_heads);
+                       as_stream(stream), slot_mapping, static_cast<const char*>(k_cache),
+                       u16(bounds), rows, num_slots, per, num_kv_heads);
   };
   pd::for_cache(head_dim, cache_type, [&](auto dim, auto e4m3) {
     go(block_bounds_kernel<dim.value, e4m3.value>);
@@ -280,22 +410,30 @@ extern "C" int pd_append_kv(const void* q, int64_t q_stride, const void* k, int6
   if (rows >= INT32_MAX / per_row - 256)
     return pd::fail(PD_EINVAL, "grid dimension exceeds device limits");
   AppendArgs p;
-  p.q = u16(q), p.k = u16(k), p.v = u16(v), p.positions = positions, p.rope = rope;
-  p.q_out = u16(q_out);
+  p.q = u16(q), p.k = u16(k), p.v = u16(v), p.rope = rope, p.q_out = u16(q_out);
   p.k_cache = static_cast<char*>(k_cache), p.v_cache = static_cast<char*>(v_cache);
-  p.slots = slot_mapping, p.k_scale = k_scale, p.v_scale = v_scale;
+  p.k_scale = k_scale, p.v_scale = v_scale, p.bounds = u16(bounds);
   p.q_stride = q_stride, p.k_stride = k_stride, p.v_stride = v_stride;
-  p.q_out_stride = q_out_stride, p.max_positions = max_positions, p.num_slots = num_slots;
-  p.rows = uint32_t(rows), p.items_per_row = uint32_t(per_row);
+  p.q_out_stride = q_out_stride, p.max_positions = max_positions;
   p.hq = num_heads, p.hkv = num_kv_heads, p.half = half;
-  const dim3 grid(unsigned((rows * per_row + 255) / 256));
+  const bool inside = bounds && rows <= kStepRows;
+  const int64_t groups =
+      (rows * per_row + 255) / 256 + (inside ? rows * int64_t(num_kv_heads) : 0);
+  if (groups > 0x7fffffff) return pd::fail(PD_EINVAL, "grid dimension exceeds device limits");
+  const auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(unsigned(groups)), dim3(256), 0, as_stream(stream),
+                       slot_mapping, positions, uint32_t(rows), uint32_t(per_row), num_slots, p);
+  };
   pd::for_cache(head_dim, cache_type, [&](auto dim, auto e4m3) {
-    const auto kernel = interleaved ? append_kernel<dim.value, e4m3.value, true>
-                                    : append_kernel<dim.value, e4m3.value, false>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, as_stream(stream), p);
+    if (inside)
+      go(interleaved ? append_kernel<dim.value, e4m3.value, true, true>
+                     : append_kernel<dim.value, e4m3.value, false, true>);
+    else
+      go(interleaved ? append_kernel<dim.value, e4m3.value, true, false>
+                     : append_kernel<dim.value, e4m3.value, false, false>);
   });
   if (const int bad = launch_status("pd_append_kv")) return bad;
-  if (!bounds) return PD_OK;
+  if (!bounds || inside) return PD_OK;
   return launch_bounds(k_cache, cache_type, num_slots, slot_mapping, rows, bounds, num_kv_heads,
                        head_dim, stream);
 }

@@ -11,8 +11,10 @@
 // A block is 64 tokens, a quarter of a page.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "pd_blocks.h"
 #include "pd_device.h"
@@ -64,212 +66,375 @@ __device__ __forceinline__ double xor_lanes64(double x, int lane) {
   return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
 }
 
-template <int kLanes>
-__device__ __forceinline__ double sum_lanes(double x, int lane) {
-  if constexpr (kLanes > 16) x += xor_lanes64<16>(x, lane);
-  if constexpr (kLanes > 8) x += xor_lanes64<8>(x, lane);
-  x += xor_lanes64<4>(x, lane);
-  x += xor_lanes64<2>(x, lane);
-  return x + xor_lanes64<1>(x, lane);
-}
-
-// A block's bounds are kLanes lanes of eight channels; a wavefront takes kRuns
-// runs of 64 / kLanes blocks, so a head's query is widened once for all of them.
+// A block's bounds are kLanes lanes of eight channels; a run is the 64 / kLanes
+// blocks of a wavefront.  kHeads query heads at a time are held as doubles.
 template <int D>
 struct Scores {
-  static constexpr int kLanes = D / 8, kPer = 64 / kLanes, kRuns = 4;
-  static constexpr int kBlocks = 4 * kRuns * kPer;  // of a workgroup
+  static constexpr int kLanes = D / 8, kPer = 64 / kLanes;
 };
 
+template <int D, int kHeads>
+struct Query {
+  double x[kHeads][8];
+  // Heads head0.. of the group; past its end the last one again, which moves no maximum.
+  __device__ __forceinline__ void load(const SelectArgs& p, int b, int g, int head0, int part) {
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      const int64_t head = int64_t(g) * p.group + min(head0 + h, p.group - 1);
+      float f[8];
+      unpack8(load16(p.q + b * p.qsb + head * p.qsh + 8 * part), f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[h][i] = f[i];
+    }
+  }
+};
+
+// Bounds of block j of sequence b, this lane's channels; a page outside the pool: known false.
 template <int D>
-__global__ void __launch_bounds__(256) score_kernel(const SelectArgs p) {
+struct Bounds {
+  u32x4_t lo, hi;
+  bool known;
+  __device__ __forceinline__ void load(const SelectArgs& p, int b, int g, int j, int part) {
+    const int64_t page = p.table[b * p.tsb + j / kPerPage];
+    known = page >= 0 && page < p.num_pages;
+    const uint16_t* at =
+        p.bounds + (((known ? page : 0) * kPerPage + j % kPerPage) * p.hkv + g) * 2 * D + 8 * part;
+    lo = load16(at);
+    hi = load16(at + D);
+  }
+};
+
+// max(q, 0) hi + min(q, 0) lo = q (hi + lo) / 2 + |q| (hi - lo) / 2, whose factors one
+// conversion of q serves; the halves are left out, they move no order.  (An infinite bound
+// gives the same infinity or NaN in both.)  The largest of kHeads heads' sums, in every
+// lane of the block: a lane pair splits the heads between them at each of the first steps,
+// so that a step moves half of the sums of the one before.
+template <int D, int kHeads>
+__device__ __forceinline__ double best_of(const Query<D, kHeads>& q, const double (&mid)[8],
+                                          const double (&radius)[8], int lane) {
+  double s[kHeads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    s[h] = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      s[h] = __builtin_fma(__builtin_fabs(q.x[h][i]), radius[i],
+                           __builtin_fma(q.x[h][i], mid[i], s[h]));
+  }
+  double x;
+  if constexpr (kHeads == 4) {
+    const bool odd = lane & 1, second = lane & 2;
+    const double a0 = (odd ? s[2] : s[0]) + xor_lanes64<1>(odd ? s[0] : s[2], lane);
+    const double a1 = (odd ? s[3] : s[1]) + xor_lanes64<1>(odd ? s[1] : s[3], lane);
+    x = (second ? a1 : a0) + xor_lanes64<2>(second ? a0 : a1, lane);
+  } else if constexpr (kHeads == 2) {
+    const bool odd = lane & 1;
+    x = (odd ? s[1] : s[0]) + xor_lanes64<1>(odd ? s[0] : s[1], lane);
+    x += xor_lanes64<2>(x, lane);
+  } else {
+    x = s[0] + xor_lanes64<1>(s[0], lane);
+    x += xor_lanes64<2>(x, lane);
+  }
+  x += xor_lanes64<4>(x, lane);
+  if constexpr (Scores<D>::kLanes > 8) x += xor_lanes64<8>(x, lane);
+  if constexpr (Scores<D>::kLanes > 16) x += xor_lanes64<16>(x, lane);
+  if (x != x) x = __builtin_inf();
+  if constexpr (kHeads > 1) x = fmax(x, xor_lanes64<1>(x, lane));
+  if constexpr (kHeads > 2) x = fmax(x, xor_lanes64<2>(x, lane));
+  return x;
+}
+
+// Scores of blocks j0 + w kPer + lane / kLanes, every `step` blocks, below `end`, to
+// store(j, key).  kHeads >= group: the query stays in registers; else it is taken again for
+// every run, kHeads heads at a time.
+template <int D, int kHeads, bool kWhole, typename Store>
+__device__ __forceinline__ void score_blocks(const SelectArgs& p, int b, int g, int j0, int step,
+                                             int end, int lane, Store store) {
   using S = Scores<D>;
+  const int part = lane % S::kLanes, mine = lane / S::kLanes;
+  if (j0 >= end) return;
+  Bounds<D> next;
+  next.load(p, b, g, min(j0 + mine, end - 1), part);
+  Query<D, kHeads> q;
+  if constexpr (kWhole) q.load(p, b, g, 0, part);
+  for (int j = j0; j < end; j += step) {
+    const Bounds<D> here = next;
+    if (j + step < end) next.load(p, b, g, min(j + step + mine, end - 1), part);
+    double mid[8], radius[8];
+    float lo[8], hi[8];
+    unpack8(here.lo, lo);
+    unpack8(here.hi, hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double l = lo[i], h = hi[i];
+      mid[i] = h + l, radius[i] = h - l;
+    }
+    double best;
+    if constexpr (kWhole) {
+      best = best_of<D, kHeads>(q, mid, radius, lane);
+    } else {
+      best = -__builtin_inf();
+      for (int head = 0; head < p.group; head += kHeads) {
+        q.load(p, b, g, head, part);
+        best = fmax(best, best_of<D, kHeads>(q, mid, radius, lane));
+      }
+    }
+    if (part == 0 && j + mine < end) store(j + mine, here.known ? score_key(best) : 0);
+  }
+}
+
+// The scores of one (sequence, kv head), cut over the workgroups of grid.x.
+template <int D, int kHeads, bool kWhole>
+__global__ void __launch_bounds__(256) score_kernel(const SelectArgs p) {
+  constexpr int kPer = Scores<D>::kPer;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int g = blockIdx.y, b = blockIdx.z;
   const int n = block_count(p.lengths, b, p.width);
-  const int end = n - p.last;
-  const int j0 = p.first + blockIdx.x * S::kBlocks + w * S::kRuns * S::kPer;
-  if (n <= p.kept || j0 >= end) return;
-  const int part = lane % S::kLanes, mine = lane / S::kLanes;
-  double lo[S::kRuns][8], hi[S::kRuns][8], best[S::kRuns];
-  bool known[S::kRuns];
-#pragma unroll
-  for (int r = 0; r < S::kRuns; ++r) {
-    const int j = min(j0 + r * S::kPer + mine, end - 1);
-    const int64_t page = p.table[b * p.tsb + j / kPerPage];
-    known[r] = page >= 0 && page < p.num_pages;
-    const uint16_t* at =
-        p.bounds + (((known[r] ? page : 0) * kPerPage + j % kPerPage) * p.hkv + g) * 2 * D + 8 * part;
-    float x[8], y[8];
-    unpack8(load16(at), x);
-    unpack8(load16(at + D), y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) lo[r][i] = x[i], hi[r][i] = y[i];
-    best[r] = -__builtin_inf();
-  }
-  const uint16_t* q = p.q + b * p.qsb + int64_t(g) * p.group * p.qsh + 8 * part;
-  for (int h = 0; h < p.group; ++h, q += p.qsh) {
-    float x[8];
-    unpack8(load16(q), x);
-    double sum[S::kRuns] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double up = x[i] != x[i] ? x[i] : fmaxf(x[i], 0.f);
-      const double down = fminf(x[i], 0.f);
-#pragma unroll
-      for (int r = 0; r < S::kRuns; ++r)
-        sum[r] = __builtin_fma(up, hi[r][i], __builtin_fma(down, lo[r][i], sum[r]));
-    }
-#pragma unroll
-    for (int r = 0; r < S::kRuns; ++r) {
-      const double s = sum_lanes<S::kLanes>(sum[r], lane);
-      best[r] = s > best[r] || s != s ? s : best[r];
-    }
-  }
-  if (part) return;
+  if (n <= p.kept) return;
   uint64_t* keys = p.keys + (int64_t(b) * p.hkv + g) * p.width * kPerPage;
+  score_blocks<D, kHeads, kWhole>(p, b, g, p.first + (blockIdx.x * 4 + w) * kPer,
+                                  gridDim.x * 4 * kPer, n - p.last, lane,
+                                  [&](int j, uint64_t key) { keys[j] = key; });
+}
+
+template <int M>
+__device__ __forceinline__ uint64_t xor_lanes_u64(uint64_t x, int lane) {
+  return __builtin_bit_cast(uint64_t, xor_lanes64<M>(__builtin_bit_cast(double, x), lane));
+}
+
+// The blocks of one (sequence, kv head) by its candidates' keys, begin <= j < end: the
+// threshold is found digit by digit from the highest bit in which the keys differ, then one
+// ordered pass writes the forced blocks, those above the threshold and the first at it.
+constexpr int kDigit = 11, kBins = 1 << kDigit;
+
+constexpr int kCached = 8;  // keys that a thread holds in its registers
+
+template <int kWaves>
+struct Picker {
+  uint32_t bins[kBins];
+  uint64_t wave_keys[2][kWaves];
+  uint64_t close_keys[64];  // the keys of the threshold's bin, where they are few
+  int32_t close_blocks[64];
+  uint32_t wave_counts[kCached][kWaves], found[2], close;
+  uint64_t edge;
+};
+
+// kCache > 0: a thread's keys, at most that many, stay in its registers.
+template <int kWaves, int kCache>
+__device__ __forceinline__ void pick_blocks(Picker<kWaves>& t, const uint64_t* __restrict__ keys,
+                                            int n, int begin, int end, uint32_t need,
+                                            int32_t* out) {
+  constexpr int kThreads = 64 * kWaves;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  uint64_t cached[kCache + 1];
 #pragma unroll
-  for (int r = 0; r < S::kRuns; ++r) {
-    const int j = j0 + r * S::kPer + mine;
-    if (j < end) keys[j] = known[r] ? score_key(best[r]) : 0;  // no such page: last
+  for (int i = 0; i < kCache; ++i) cached[i] = keys[min(begin + tid + i * kThreads, end - 1)];
+  const auto each = [&](auto use) {  // use(j, key) of the thread's candidates
+    if constexpr (kCache > 0) {
+#pragma unroll
+      for (int i = 0; i < kCache; ++i)
+        if (begin + i * kThreads < end) {
+          const int j = begin + tid + i * kThreads;
+          if (j < end) use(j, cached[i]);
+        }
+    } else {
+      for (int j = begin + tid; j < end; j += kThreads) use(j, keys[j]);
+    }
+  };
+  for (int i = tid; i < kBins; i += kThreads) t.bins[i] = 0;
+  if (tid == 0) t.close = 0;
+  uint64_t every = ~uint64_t(0), some = 0;
+  each([&](int, uint64_t key) { every &= key, some |= key; });
+  every &= xor_lanes_u64<1>(every, lane), some |= xor_lanes_u64<1>(some, lane);
+  every &= xor_lanes_u64<2>(every, lane), some |= xor_lanes_u64<2>(some, lane);
+  every &= xor_lanes_u64<4>(every, lane), some |= xor_lanes_u64<4>(some, lane);
+  every &= xor_lanes_u64<8>(every, lane), some |= xor_lanes_u64<8>(some, lane);
+  every &= xor_lanes_u64<16>(every, lane), some |= xor_lanes_u64<16>(some, lane);
+  every &= xor_lanes_u64<32>(every, lane), some |= xor_lanes_u64<32>(some, lane);
+  if (lane == 0) t.wave_keys[0][w] = every, t.wave_keys[1][w] = some;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) every &= t.wave_keys[0][i], some |= t.wave_keys[1][i];
+
+  // Keys whose bits from `shift` (below 64) up are above `edge` are in, and `need` of those
+  // at it.
+  const uint64_t differ = every ^ some;
+  int shift = differ ? 64 - __builtin_clzll(differ) : 0;
+  uint64_t edge = shift < 64 ? some >> shift : 0;
+  uint32_t at_edge = end - begin;
+  const uint32_t taken = need;
+  if (need == 0) edge = ~uint64_t(0), shift = 0;
+  bool clear = true;  // bins
+  while (need && shift > 0 && at_edge != need) {
+    if (!clear && at_edge <= 64) {
+      // Few keys share the edge: the need-th of them by their ranks.
+      each([&](int j, uint64_t key) {
+        if (key >> shift == edge) {
+          const uint32_t at = atomicAdd(&t.close, 1u);
+          t.close_keys[at] = key, t.close_blocks[at] = j;
+        }
+      });
+      __syncthreads();
+      if (w == 0) {
+        const uint64_t key = t.close_keys[lane];
+        const int j = t.close_blocks[lane];
+        uint32_t above = 0, same = 0;
+        for (uint32_t i = 0; i < at_edge; ++i) {
+          above += t.close_keys[i] > key;
+          same += t.close_keys[i] == key && t.close_blocks[i] < j;
+        }
+        if (lane < int(at_edge) && above + same == need - 1) t.edge = key, t.found[0] = same + 1;
+      }
+      __syncthreads();
+      edge = t.edge, need = t.found[0], shift = 0;
+      break;
+    }
+    const int next = max(shift - kDigit, 0);
+    if (!clear) {
+      for (int i = tid; i < kBins; i += kThreads) t.bins[i] = 0;
+      __syncthreads();
+    }
+    clear = false;
+    each([&](int, uint64_t key) {
+      if ((shift < 64 ? key >> shift : 0) == edge)
+        atomicAdd(&t.bins[(key >> next) & ((1u << (shift - next)) - 1)], 1u);
+    });
+    __syncthreads();
+    // From the highest bin down: the one in which the count reaches `need`.
+    constexpr int kOwn = kBins / kThreads;
+    const int top = kBins - 1 - tid * kOwn;
+    uint32_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) sum += t.bins[top - i];
+    uint32_t before = sum;
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const uint32_t x = __shfl_up(before, m);
+      if (lane >= m) before += x;
+    }
+    if (lane == 63) t.wave_counts[0][w] = before;
+    __syncthreads();
+    for (int i = 0; i < w; ++i) before += t.wave_counts[0][i];
+    before -= sum;
+    if (before < need && before + sum >= need) {
+      uint32_t above = before;
+      int bin = top;
+      while (above + t.bins[bin] < need) above += t.bins[bin--];
+      t.found[0] = bin, t.found[1] = above;
+    }
+    __syncthreads();
+    const uint32_t bin = t.found[0];
+    need -= t.found[1];
+    at_edge = t.bins[bin];
+    edge = (shift < 64 ? edge << (shift - next) : 0) | bin;
+    shift = next;
+    __syncthreads();
+  }
+
+  for (int j = tid; j < begin; j += kThreads) out[j] = j;
+  for (int i = tid; i < n - end; i += kThreads) out[begin + taken + i] = end + i;
+  // In order: kWave threads' blocks at a time, a thread's place by the counts ahead of it.
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+  uint32_t written = begin, ties = 0;
+  const auto marks = [&](int j, uint64_t key, bool& in, bool& tie) {
+    if (shift < 64) key >>= shift;
+    in = j < end && shift < 64 && key > edge;
+    tie = j < end && (shift == 64 || key == edge);
+  };
+  const auto place = [&](int j, bool in, bool tie, const uint32_t (&counts)[kWaves]) {
+    uint32_t ahead = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      if (i < w) ahead += counts[i];
+      all += counts[i];
+    }
+    // Ties ahead of this block that are in: the first `need` of them.
+    const uint32_t tied = ties + (ahead >> 16) + __popcll(__ballot(tie) & below);
+    const uint32_t at = written + (ahead & 0xffff) + __popcll(__ballot(in) & below) + min(tied, need);
+    if (in || (tie && tied < need)) out[at] = j;
+    written += all & 0xffff;
+    ties += all >> 16;
+  };
+  const auto count = [&](bool in, bool tie, uint32_t& cell) {
+    const uint32_t both = uint32_t(__popcll(__ballot(in))) | uint32_t(__popcll(__ballot(tie))) << 16;
+    if (lane == 0) cell = both;
+  };
+  bool in, tie;
+  if constexpr (kCache > 0) {
+#pragma unroll
+    for (int i = 0; i < kCache; ++i)
+      if (begin + i * kThreads < end) {
+        marks(begin + tid + i * kThreads, cached[i], in, tie);
+        count(in, tie, t.wave_counts[i][w]);
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kCache; ++i)
+      if (begin + i * kThreads < end) {
+        marks(begin + tid + i * kThreads, cached[i], in, tie);
+        place(begin + tid + i * kThreads, in, tie, t.wave_counts[i]);
+      }
+  } else {
+    for (int base = begin; base < end; base += kThreads) {
+      marks(base + tid, keys[min(base + tid, end - 1)], in, tie);
+      count(in, tie, t.wave_counts[0][w]);
+      __syncthreads();
+      place(base + tid, in, tie, t.wave_counts[0]);
+      __syncthreads();
+    }
   }
 }
 
-// The r highest keys of a (sequence, kv head): the threshold found digit by
-// digit from the highest bit in which the keys differ, then one ordered pass
-// that writes the forced blocks, those above the threshold and the first ones at
-// it.
-constexpr int kDigit = 11, kBins = 1 << kDigit;
+__device__ __forceinline__ void list_all(int32_t* out, int kept, int n) {
+  for (int i = threadIdx.x; i < kept; i += blockDim.x) out[i] = i < n ? i : -1;
+}
 
-__global__ void __launch_bounds__(256) pick_kernel(const SelectArgs p) {
-  __shared__ uint32_t bins[kBins];
-  __shared__ uint64_t wave_keys[2][4];
-  __shared__ uint32_t wave_counts[4], found[2];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+// One sequence of 512 blocks: 7.7 us for both launches with 4 wavefronts, 8.0 with 8, 9.4 with
+// 16, whose barriers cost more than their keys.
+constexpr int kPickWaves = 4;
+
+__global__ void __launch_bounds__(64 * kPickWaves) pick_kernel(const SelectArgs p) {
+  __shared__ Picker<kPickWaves> picker;
   const int g = blockIdx.x, b = blockIdx.y;
   const int n = block_count(p.lengths, b, p.width);
   int32_t* out = p.blocks + (int64_t(b) * p.hkv + g) * p.kept;
-  if (n <= p.kept) {
-    for (int i = tid; i < p.kept; i += 256) out[i] = i < n ? i : -1;
-    return;
-  }
+  if (n <= p.kept) return list_all(out, p.kept, n);
   const uint64_t* keys = p.keys + (int64_t(b) * p.hkv + g) * p.width * kPerPage;
   const int begin = p.first, end = n - p.last;
-  uint32_t need = p.kept - p.first - p.last;  // < end - begin
-  uint64_t every = ~uint64_t(0), some = 0;
-  for (int j = begin + tid; j < end; j += 256) every &= keys[j], some |= keys[j];
-  for (int m = 1; m < 64; m *= 2) {
-    every &= __shfl_xor(every, m);
-    some |= __shfl_xor(some, m);
-  }
-  if (lane == 0) wave_keys[0][w] = every, wave_keys[1][w] = some;
-  __syncthreads();
-  every = wave_keys[0][0] & wave_keys[0][1] & wave_keys[0][2] & wave_keys[0][3];
-  some = wave_keys[1][0] | wave_keys[1][1] | wave_keys[1][2] | wave_keys[1][3];
-
-  // Keys above `edge` (of the bits at `shift` and up) are in; `need` of those at it.
-  uint64_t edge = 0;
-  const uint64_t differ = every ^ some;
-  int shift = differ ? 64 - __builtin_clzll(differ) : 0;
-  uint32_t at_edge = end - begin;  // keys that agree with the edge so far
-  edge = shift < 64 ? some >> shift : 0;
-  if (need == 0) {
-    edge = ~uint64_t(0), shift = 0, at_edge = 0;
-  } else {
-    while (shift > 0 && at_edge != need) {
-      const int next = max(shift - kDigit, 0);
-      for (int i = tid; i < kBins; i += 256) bins[i] = 0;
-      __syncthreads();
-      for (int j = begin + tid; j < end; j += 256) {
-        const uint64_t key = keys[j];
-        if ((shift < 64 ? key >> shift : 0) == edge)
-          atomicAdd(&bins[(key >> next) & ((1u << (shift - next)) - 1)], 1u);
-      }
-      __syncthreads();
-      // From the highest bin down: the one in which the count reaches `need`.
-      uint32_t sum = 0;
-      constexpr int kOwn = kBins / 256;
-      const int top = kBins - 1 - tid * kOwn;
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) sum += bins[top - i];
-      uint32_t before = sum;
-      for (int m = 1; m < 64; m *= 2) {
-        const uint32_t x = __shfl_up(before, m);
-        if (lane >= m) before += x;
-      }
-      if (lane == 63) wave_counts[w] = before;
-      __syncthreads();
-      for (int i = 0; i < w; ++i) before += wave_counts[i];
-      before -= sum;
-      if (before < need && before + sum >= need) {
-        uint32_t above = before;
-        int bin = top;
-        while (above + bins[bin] < need) above += bins[bin--];
-        found[0] = bin, found[1] = above;
-      }
-      __syncthreads();
-      const uint32_t bin = found[0];
-      need -= found[1];
-      at_edge = bins[bin];
-      edge = (shift < 64 ? edge << (shift - next) : 0) | bin;
-      shift = next;
-      __syncthreads();
-    }
-  }
-  uint32_t written = 0, ties = 0;
-  for (int base = 0; base < n; base += 256) {
-    const int j = base + tid;
-    bool in = j < n && (j < begin || j >= end), tie = false;
-    if (j >= begin && j < end) {
-      const uint64_t key = shift < 64 ? keys[j] >> shift : 0;
-      in = key > edge;
-      tie = key == edge;
-    }
-    const uint64_t below = (uint64_t(1) << lane) - 1;
-    const uint64_t mask_in = __ballot(in), mask_tie = __ballot(tie);
-    __syncthreads();
-    if (lane == 0)
-      wave_counts[w] = uint32_t(__popcll(mask_in)) | uint32_t(__popcll(mask_tie)) << 16;
-    __syncthreads();
-    uint32_t ahead = 0, all = 0;
-    for (int i = 0; i < 4; ++i) {
-      if (i < w) ahead += wave_counts[i];
-      all += wave_counts[i];
-    }
-    // Ties ahead of this block that are in: the first `need` of them.
-    const uint32_t tied = ties + (ahead >> 16) + __popcll(mask_tie & below);
-    const uint32_t place = written + (ahead & 0xffff) + __popcll(mask_in & below) + min(tied, need);
-    if (in || (tie && tied < need)) out[place] = j;
-    written += all & 0xffff;
-    ties += all >> 16;
-  }
+  const uint32_t need = uint32_t(p.kept - p.first - p.last);
+  if (end - begin <= kCached * 64 * kPickWaves)
+    pick_blocks<kPickWaves, kCached>(picker, keys, n, begin, end, need, out);
+  else
+    pick_blocks<kPickWaves, 0>(picker, keys, n, begin, end, need, out);
 }
 
 // ------------------------------------------------------------------ attention
 
 struct DecodeArgs {
-  const uint16_t* q;
-  const char *k, *v;
-  const int32_t *table, *lengths, *blocks;  // blocks null: every block
   const float *k_scale, *v_scale;
   float *part_o, *part_ml;  // [batch][heads][splits][D], [batch][heads][splits][2]
   uint16_t* out;
-  int64_t qsb, qsh, tsb, num_pages;
-  int width, hkv, group, tiles, kept, splits;  // tiles: of 16 query heads a kv head
-  float scale2;                                // scale log2 e
+  int64_t qsb, qsh;
+  int group, tiles;  // tiles: of 16 query heads a kv head
+  float scale2;      // scale log2 e
 };
 
-// A wavefront's tile: 32 tokens.  S^T = K Q^T and O^T = V^T P^T with 16 x 16 x 32
-// MFMAs.  In both results a lane's column is query head lane % 16, so the softmax
-// state is one scalar a lane, and the layout of the scores (tokens 16 u + 4 (lane /
-// 16) + r in element r of half u) is the operand layout of P^T with its tokens in
-// that order, which V's rows are loaded in too.  V^T's operand wants eight tokens
-// of a channel in a lane: a lane loads kRun channels of eight tokens and turns the
-// 8 x kRun square with byte permutes; row m of the MFMA of channel j is channel
-// kRun m + j.  No value crosses a lane or the LDS before the end.
+// A wavefront's tile: kTile tokens, 8 KB of K and of V (at most 64 tokens).  S^T = K Q^T and
+// O^T = V^T P^T with 16 x 16 x 32 MFMAs.  In both results a lane's column is query head
+// lane % 16, so the softmax state is one scalar a lane, and the layout of the scores (tokens
+// 16 u + 4 (lane / 16) + r in element r of result u) is the operand layout of P^T with its
+// tokens in that order, which V's rows are loaded in too.  V^T's operand wants eight tokens
+// of a channel in a lane: a lane loads kRun channels of eight tokens and turns the 8 x kRun
+// square with byte permutes; row m of the MFMA of channel j is channel kRun m + j.  No value
+// crosses a lane or the LDS before the end.  A bf16 tile at head_dim 256 is 16 tokens, its
+// P V MFMAs 16 x 16 x 16.
 template <int D, bool kE4m3>
 struct Decode {
   static constexpr int kBytes = kE4m3 ? 1 : 2;
+  static constexpr int kTile = D * kBytes >= 512 ? 16 : D * kBytes >= 256 ? 32 : 64;
+  static constexpr int kSums = kTile / 16;               // results of S^T
+  static constexpr int kGroups = kTile < 32 ? 1 : kTile / 32;
+  static constexpr int kPer = kTile < 32 ? 4 : 8;        // tokens of a lane's P V operand
   static constexpr int kStepsQ = D / 32;
   static constexpr int kKLoads = D * kBytes / 64;        // 16-byte loads a lane and 16 tokens
   static constexpr int kRun = D / 16 < 16 / kBytes ? D / 16 : 16 / kBytes;  // channels a load
@@ -281,6 +446,10 @@ struct Decode {
   static __device__ __forceinline__ int channel(int s, int row) {
     return kE4m3 ? (s / 2) * 64 + row * 16 + (s % 2) * 8 : s * 32 + row * 8;
   }
+  // Token of element i of group a's operand.
+  static __device__ __forceinline__ int token(int a, int i, int row) {
+    return 32 * a + 16 * (i >> 2) + 4 * row + (i & 3);
+  }
 };
 
 template <int N>
@@ -288,18 +457,28 @@ struct Words {
   uint32_t w[N];
 };
 
-template <int N>
+// Rows of 512 bytes pass the caches by; the lines of shorter ones are still to be read by
+// another load.
+template <typename V, int kRowBytes>
+__device__ __forceinline__ V load_row(const char* p) {
+  if constexpr (kRowBytes >= 512)
+    return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+  else
+    return *reinterpret_cast<const V*>(p);
+}
+
+template <int N, int kRowBytes>
 __device__ __forceinline__ Words<N> load_words(const char* p) {
   Words<N> r;
   if constexpr (N == 4) {
-    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(p);
+    const u32x4_t x = load_row<u32x4_t, kRowBytes>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) r.w[i] = x[i];
   } else if constexpr (N == 2) {
-    const u32x2_t x = *reinterpret_cast<const u32x2_t*>(p);
+    const u32x2_t x = load_row<u32x2_t, kRowBytes>(p);
     r.w[0] = x[0], r.w[1] = x[1];
   } else {
-    r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+    r.w[0] = load_row<uint32_t, kRowBytes>(p);
   }
   return r;
 }
@@ -310,30 +489,45 @@ __device__ __forceinline__ uint32_t e4m3_to_bf16(uint32_t x) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, kUpper));
 }
 
+typedef short short4v_t __attribute__((ext_vector_type(4)));
+
+// D += A B over kPer tokens a lane.
+template <int kPer>
+__device__ __forceinline__ floatx4_t mfma_pv(const Words<kPer / 2>& a, const Words<kPer / 2>& b,
+                                             floatx4_t c) {
+  if constexpr (kPer == 8)
+    return mfma16(__builtin_bit_cast(u32x4_t, a), __builtin_bit_cast(u32x4_t, b), c);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4v_t, a),
+                                                     __builtin_bit_cast(short4v_t, b), c, 0, 0, 0);
+}
+
 template <int D, bool kE4m3>
 struct Tile {
   using T = Decode<D, kE4m3>;
-  u32x4_t k[2][T::kKLoads];
-  Words<T::kWords> v[T::kChunks][8];
+  u32x4_t k[T::kSums][T::kKLoads];
+  Words<T::kWords> v[T::kGroups][T::kChunks][T::kPer];
 
-  // `token`: bytes between tokens; rows of 32 tokens at `base`.
+  // Rows of kTile tokens at `base`, `token` bytes apart.
   __device__ __forceinline__ void load_k(const char* base, uint32_t token, int lane) {
     const uint32_t at = uint32_t(lane & 15) * token + uint32_t(lane >> 4) * 16;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < T::kSums; ++u)
 #pragma unroll
       for (int i = 0; i < T::kKLoads; ++i)
-        k[u][i] = *reinterpret_cast<const u32x4_t*>(base + (at + u * 16 * token + i * 64));
+        k[u][i] = load_row<u32x4_t, D * T::kBytes>(base + (at + u * 16 * token + i * 64));
   }
   __device__ __forceinline__ void load_v(const char* base, uint32_t token, int lane) {
     const uint32_t at =
         uint32_t(lane >> 4) * 4 * token + uint32_t(lane & 15) * T::kRun * T::kBytes;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int a = 0; a < T::kGroups; ++a)
 #pragma unroll
-      for (int c = 0; c < T::kChunks; ++c)
-        v[c][i] = load_words<T::kWords>(
-            base + (at + ((i & 3) + 16 * (i >> 2)) * token + c * 16 * T::kRun * T::kBytes));
+      for (int i = 0; i < T::kPer; ++i)
+#pragma unroll
+        for (int c = 0; c < T::kChunks; ++c)
+          v[a][c][i] = load_words<T::kWords, D * T::kBytes>(
+              base + (at + T::token(a, i, 0) * token + c * 16 * T::kRun * T::kBytes));
   }
   __device__ __forceinline__ u32x4_t k_operand(int u, int s) const {
     if constexpr (kE4m3) {
@@ -345,48 +539,64 @@ struct Tile {
     }
   }
   // Channel j of chunk c, tokens in the order of the scores.
-  __device__ __forceinline__ u32x4_t v_operand(int c, int j) const {
-    u32x4_t r;
+  __device__ __forceinline__ Words<T::kPer / 2> v_operand(int group, int c, int j) const {
+    Words<T::kPer / 2> r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < T::kPer / 2; ++i) {
       uint32_t a, b;
       if constexpr (kE4m3) {
-        a = (j & 2) ? e4m3_to_bf16<true>(v[c][2 * i].w[j / 4])
-                    : e4m3_to_bf16<false>(v[c][2 * i].w[j / 4]);
-        b = (j & 2) ? e4m3_to_bf16<true>(v[c][2 * i + 1].w[j / 4])
-                    : e4m3_to_bf16<false>(v[c][2 * i + 1].w[j / 4]);
+        const uint32_t x = v[group][c][2 * i].w[j / 4], y = v[group][c][2 * i + 1].w[j / 4];
+        a = (j & 2) ? e4m3_to_bf16<true>(x) : e4m3_to_bf16<false>(x);
+        b = (j & 2) ? e4m3_to_bf16<true>(y) : e4m3_to_bf16<false>(y);
       } else {
-        a = v[c][2 * i].w[j / 2], b = v[c][2 * i + 1].w[j / 2];
+        a = v[group][c][2 * i].w[j / 2], b = v[group][c][2 * i + 1].w[j / 2];
       }
-      r[i] = __builtin_amdgcn_perm(b, a, (j & 1) ? 0x07060302u : 0x05040100u);
+      r.w[i] = __builtin_amdgcn_perm(b, a, (j & 1) ? 0x07060302u : 0x05040100u);
     }
     return r;
   }
 };
 
+// The leading arguments are in registers when a wavefront starts, the others are loaded
+// while the length and the table are.
 template <int D, bool kE4m3>
-__global__ void __launch_bounds__(256) block_decode_kernel(const DecodeArgs p) {
+__global__ void __launch_bounds__(256, D == 128 && !kE4m3 ? 3 : 2)
+block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restrict__ blocks,
+                    const int32_t* __restrict__ table, int64_t tsb, int width, int kept, int hkv,
+                    int num_pages, const char* __restrict__ k, const char* __restrict__ v,
+                    const uint16_t* __restrict__ q_rows, const DecodeArgs p) {
   using T = Decode<D, kE4m3>;
-  extern __shared__ float shared[];  // [4][16][2] (m, l), then [4][heads][D]
+  constexpr int kTile = T::kTile, kTiles = pd::kPageSize / kTile, kParts = kBlock / kTile;
+  extern __shared__ floatx4_t shared[];  // [4][16] (m, l) pairs, then [4][kOut][4][heads]
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = lane >> 4, col = lane & 15;
-  // Kv heads of a sequence's split are neighbours: their rows of a token are too.
-  int id = blockIdx.x;
-  const int tile = id % p.tiles;
-  id /= p.tiles;
-  const int g = id % p.hkv;
-  id /= p.hkv;
-  const int split = id % p.splits, b = id / p.splits;
-  const int heads = min(p.group - 16 * tile, 16);
-  const int head0 = g * p.group + 16 * tile;
+  int x = blockIdx.x, split = blockIdx.y, b = blockIdx.z;
+  const int splits = gridDim.y;
+  // Workgroups of neighbouring x go to the XCDs in turn.  Where two heads' rows share a
+  // 128-byte line, those of such a pair are eight apart, so that one XCD's L2 reads the line
+  // once.
+  constexpr int kPair = D * T::kBytes < 128 ? 2 : 1;
+  if constexpr (kPair == 2) {
+    const uint32_t all = gridDim.x * gridDim.y * gridDim.z;
+    uint32_t id = x + gridDim.x * (split + gridDim.y * b);
+    if ((id | 15) < all) id = (id & ~15u) | (id & 7) * 2 | (id >> 3 & 1);
+    x = id % gridDim.x, id /= gridDim.x;
+    split = id % gridDim.y, b = id / gridDim.y;
+  }
+  // With a head on the same XCD throughout, the rows that an XCD reads lie a token apart, in
+  // few of its L2's channels: the heads take turns.
+  x = uint32_t(x + kPair * (split + b)) % gridDim.x;
+  int g = x, head_tile = 0;
+  if (int(gridDim.x) != hkv) g = x / p.tiles, head_tile = x % p.tiles;
+  const int heads = min(p.group - 16 * head_tile, 16);
+  const int head0 = g * p.group + 16 * head_tile;
 
-  // Whole blocks of the list a split, the same for each of a sequence's splits; a
-  // multiple of 4, so that no wavefront gets more than the others' and one.
-  const int64_t len = min(int64_t(max(p.lengths[b], 0)), int64_t(p.width) * pd::kPageSize);
-  int entries = int((len + kBlock - 1) / kBlock);
-  if (p.blocks) entries = min(entries ? p.kept : 0, p.kept);
-  const int chunk = ((entries + p.splits - 1) / p.splits + 3) & ~3;
-  const int s0 = split * chunk, s1 = min(s0 + chunk, entries);
+  // Tiles of the sequence, parts of its blocks or of the listed ones.  A split is whole
+  // rounds of the four wavefronts, the same for each of a sequence's splits.
+  const int64_t len = min(int64_t(max(lengths[b], 0)), int64_t(width) * pd::kPageSize);
+  const int count = blocks ? kParts * kept : int((len + kTile - 1) / kTile);
+  const int chunk = ((count + splits - 1) / splits + 3) & ~3;
+  const int s0 = split * chunk, s1 = min(s0 + chunk, count);
 
   floatx4_t o[T::kOut];
 #pragma unroll
@@ -395,180 +605,236 @@ __global__ void __launch_bounds__(256) block_decode_kernel(const DecodeArgs p) {
 
   if (s0 < s1) {
     u32x4_t q[T::kStepsQ];
-    const uint16_t* qrow = p.q + b * p.qsb + (head0 + min(col, heads - 1)) * p.qsh;
+    const uint16_t* qrow = q_rows + b * p.qsb + (head0 + min(col, heads - 1)) * p.qsh;
 #pragma unroll
     for (int s = 0; s < T::kStepsQ; ++s) q[s] = load16(qrow + T::channel(s, row));
     const float scale2 = p.scale2 * (kE4m3 && p.k_scale ? p.k_scale[g] : 1.f);
-    const uint32_t token = uint32_t(p.hkv) * D * T::kBytes;
+    const uint32_t token = uint32_t(hkv) * D * T::kBytes;
 
     // One tile: scores of the loaded K, then the next tile's K is on its way
     // while the softmax and P V run, and its V while its scores do.
     Tile<D, kE4m3> t;
     const auto step = [&](int live, auto next_k, auto next_v) {
-      floatx4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      floatx4_t s[T::kSums];
 #pragma unroll
-      for (int i = 0; i < T::kStepsQ; ++i) {
-        s[0] = mfma16(t.k_operand(0, i), q[i], s[0]);
-        s[1] = mfma16(t.k_operand(1, i), q[i], s[1]);
-      }
+      for (int u = 0; u < T::kSums; ++u) s[u] = floatx4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < T::kStepsQ; ++i)
+#pragma unroll
+        for (int u = 0; u < T::kSums; ++u) s[u] = mfma16(t.k_operand(u, i), q[i], s[u]);
       next_k();
-      float x[8], top = m;
+      float x[T::kGroups][T::kPer], top = m;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * scale2;
-      if (live < 32) {
+      for (int a = 0; a < T::kGroups; ++a)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const bool in = 16 * (i >> 2) + 4 * row + (i & 3) < live;
-          x[i] = in ? x[i] : -INFINITY;
-          // A zero probability must not meet an infinity or NaN.
+        for (int i = 0; i < T::kPer; ++i) x[a][i] = s[2 * a + (i >> 2)][i & 3] * scale2;
+      if (live < kTile) {
 #pragma unroll
-          for (int c = 0; c < T::kChunks; ++c)
+        for (int a = 0; a < T::kGroups; ++a)
 #pragma unroll
-            for (int e = 0; e < T::kWords; ++e) t.v[c][i].w[e] = in ? t.v[c][i].w[e] : 0u;
-        }
+          for (int i = 0; i < T::kPer; ++i) {
+            const bool in = T::token(a, i, row) < live;
+            x[a][i] = in ? x[a][i] : -INFINITY;
+            // A zero probability must not meet an infinity or NaN.
+#pragma unroll
+            for (int c = 0; c < T::kChunks; ++c)
+#pragma unroll
+              for (int e = 0; e < T::kWords; ++e)
+                t.v[a][c][i].w[e] = in ? t.v[a][c][i].w[e] : 0u;
+          }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
+      for (int a = 0; a < T::kGroups; ++a)
+#pragma unroll
+        for (int i = 0; i < T::kPer; ++i) top = fmaxf(top, x[a][i]);
       top = max_rows(top);
       const float base = top == -INFINITY ? 0.f : top;  // no score yet: exp2(-inf) = 0
       const float shrink = exp2_fast(m - base);
       m = top;
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i] = exp2_fast(x[i] - base);
-        sum += x[i];
-      }
-      l = l * shrink + sum;
-      // p = hi + lo to 16 significant bits: bf16 probabilities alone would add an
-      // error as large as the output's own rounding.
-      u32x4_t hi, lo;
+      for (int a = 0; a < T::kGroups; ++a)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t a = __float_as_uint(x[2 * i]), c = __float_as_uint(x[2 * i + 1]);
-        hi[i] = __builtin_amdgcn_perm(c, a, 0x07060302u);
-        lo[i] = pack_bf16(x[2 * i] - __uint_as_float(a & 0xffff0000u),
-                          x[2 * i + 1] - __uint_as_float(c & 0xffff0000u));
-      }
+        for (int i = 0; i < T::kPer; ++i) {
+          x[a][i] = exp2_fast(x[a][i] - base);
+          sum += x[a][i];
+        }
+      l = l * shrink + sum;
       if (__any(shrink != 1.f)) {
 #pragma unroll
         for (int i = 0; i < T::kOut; ++i) o[i] *= shrink;
       }
 #pragma unroll
-      for (int c = 0; c < T::kChunks; ++c)
+      for (int a = 0; a < T::kGroups; ++a) {
+        // p = hi + lo to 16 significant bits: bf16 probabilities alone would add an
+        // error as large as the output's own rounding.
+        Words<T::kPer / 2> hi, lo;
 #pragma unroll
-        for (int j = 0; j < T::kRun; ++j) {
-          const u32x4_t a = t.v_operand(c, j);
-          o[c * T::kRun + j] = mfma16(a, lo, o[c * T::kRun + j]);
-          o[c * T::kRun + j] = mfma16(a, hi, o[c * T::kRun + j]);
+        for (int i = 0; i < T::kPer / 2; ++i) {
+          const float x0 = x[a][2 * i], x1 = x[a][2 * i + 1];
+          const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
+          hi.w[i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+          lo.w[i] = pack_bf16(x0 - __uint_as_float(b0 & 0xffff0000u),
+                              x1 - __uint_as_float(b1 & 0xffff0000u));
         }
+#pragma unroll
+        for (int c = 0; c < T::kChunks; ++c)
+#pragma unroll
+          for (int j = 0; j < T::kRun; ++j) {
+            const Words<T::kPer / 2> operand = t.v_operand(a, c, j);
+            o[c * T::kRun + j] = mfma_pv<T::kPer>(operand, lo, o[c * T::kRun + j]);
+            o[c * T::kRun + j] = mfma_pv<T::kPer>(operand, hi, o[c * T::kRun + j]);
+          }
+      }
       next_v();
     };
 
-    // Entries w, w + 4, ... of the split, 64 at a time, one a lane: its page and
+    // Tiles w, w + 4, ... of the split, 64 at a time, one a lane: its first slot / kTile and
     // its live tokens (none: no such block or page).
     for (int at = s0 + w; at < s1; at += 4 * 64) {
-      const int i = at + 4 * lane;
-      int page = 0, live = 0, quarter = 0;
-      if (i < s1) {
-        const int j = p.blocks ? p.blocks[(int64_t(b) * p.hkv + g) * p.kept + i] : i;
-        const int64_t left = len - int64_t(j) * kBlock;
+      const int u = at + 4 * lane;
+      int first = 0, live = 0;
+      if (u < s1) {
+        const int64_t j = blocks ? kParts * int64_t(blocks[(int64_t(b) * hkv + g) * kept + u / kParts]) +
+                                       u % kParts
+                                 : u;
+        const int64_t left = len - j * kTile;
         if (j >= 0 && left > 0) {
-          page = p.table[b * p.tsb + j / kPerPage];
-          quarter = j % kPerPage;
-          live = page >= 0 && page < p.num_pages ? int(min(left, int64_t(kBlock))) : 0;
-          if (!live) page = 0;
+          const int page = table[b * tsb + uint32_t(j) / kTiles];
+          if (page >= 0 && page < num_pages) {
+            first = page * kTiles + int(uint32_t(j) % kTiles);
+            live = left < kTile ? int(left) : kTile;
+          }
         }
       }
       const uint64_t any = __ballot(live > 0);
       if (!any) continue;
       const int last = 63 - __builtin_clzll(any);
-      // Of tile u: entry u / 2, its first or second 32 tokens.
-      const auto offset = [&](int u) {
-        const int64_t pg = __builtin_amdgcn_readlane(page, u >> 1);
-        const int qt = __builtin_amdgcn_readlane(quarter, u >> 1);
-        return ((pg * kPerPage + qt) * kBlock + 32 * (u & 1)) * token + int64_t(g) * D * T::kBytes;
+      const auto offset = [&](int i) {
+        return int64_t(uint32_t(__builtin_amdgcn_readlane(first, i))) * kTile * token +
+               int64_t(g) * D * T::kBytes;
       };
-      const auto tokens = [&](int u) {
-        return __builtin_amdgcn_readlane(live, u >> 1) - 32 * (u & 1);
-      };
-      const int tiles = 2 * last + (tokens(2 * last + 1) > 0 ? 2 : 1);
       int64_t here = offset(0);
-      t.load_k(p.k + here, token, lane);
-      t.load_v(p.v + here, token, lane);
-      for (int u = 0; u + 1 < tiles; ++u) {
-        here = offset(u + 1);
-        step(tokens(u), [&] { t.load_k(p.k + here, token, lane); },
-             [&] { t.load_v(p.v + here, token, lane); });
+      t.load_k(k + here, token, lane);
+      t.load_v(v + here, token, lane);
+      for (int i = 0; i < last; ++i) {
+        here = offset(i + 1);
+        step(__builtin_amdgcn_readlane(live, i), [&] { t.load_k(k + here, token, lane); },
+             [&] { t.load_v(v + here, token, lane); });
       }
-      step(tokens(tiles - 1), [] {}, [] {});
+      step(__builtin_amdgcn_readlane(live, last), [] {}, [] {});
     }
     l = sum_rows(l);
   }
 
   // The four wavefronts' sums, relative to their largest maximum.
-  float* ml = shared;
-  float* part = shared + 128;
+  float* ml = reinterpret_cast<float*>(shared);
+  floatx4_t* part = shared + 32;
   if (row == 0) ml[(w * 16 + col) * 2] = m, ml[(w * 16 + col) * 2 + 1] = l;
   __syncthreads();
-  float top = -INFINITY, total = 0.f;
+  float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[(i * 16 + col) * 2]);
-  const float base = top == -INFINITY ? 0.f : top;
   if (col < heads) {
-    const float f = exp2_fast(m - base);
+    const float f = exp2_fast(m - (top == -INFINITY ? 0.f : top));
 #pragma unroll
-    for (int c = 0; c < T::kChunks; ++c)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < T::kRun; ++j)
-          part[(w * heads + col) * D + (c * 16 + 4 * row + r) * T::kRun + j] =
-              o[c * T::kRun + j][r] * f;
+    for (int i = 0; i < T::kOut; ++i) part[((w * T::kOut + i) * 4 + row) * heads + col] = o[i] * f;
   }
   __syncthreads();
-  const int64_t first = int64_t(b) * p.hkv * p.group + head0;
+  const int64_t first = int64_t(b) * hkv * p.group + head0;
   for (int i = threadIdx.x; i < heads * D / 4; i += 256) {
     const int h = i / (D / 4), d = 4 * (i % (D / 4));
     float hm = -INFINITY, hl = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) hm = fmaxf(hm, ml[(k * 16 + h) * 2]);
+    for (int j = 0; j < 4; ++j) hm = fmaxf(hm, ml[(j * 16 + h) * 2]);
     const float hb = hm == -INFINITY ? 0.f : hm;
+    // Channels d..d+3 are channels j.. of row m of their chunk's MFMAs.
+    const int row_m = d / T::kRun, j0 = row_m / 16 * T::kRun + d % T::kRun;
+    const float* cell = reinterpret_cast<const float*>(part + ((j0 * 4 + row_m % 16 / 4) * heads + h)) +
+                        row_m % 4;
     floatx4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      hl += ml[(k * 16 + h) * 2 + 1] * exp2_fast(ml[(k * 16 + h) * 2] - hb);
-      sum += *reinterpret_cast<const floatx4_t*>(part + (k * heads + h) * D + d);
+    for (int j = 0; j < 4; ++j) {
+      hl += ml[(j * 16 + h) * 2 + 1] * exp2_fast(ml[(j * 16 + h) * 2] - hb);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += cell[(j * T::kOut + e) * 16 * heads];
     }
-    if (p.splits == 1) {
-      const float scale = (kE4m3 && p.v_scale ? p.v_scale[g] : 1.f) / (hl == 0.f ? 1.f : hl);
-      sum *= scale;
+    if (splits == 1) {
+      sum *= (kE4m3 && p.v_scale ? p.v_scale[g] : 1.f) / (hl == 0.f ? 1.f : hl);
       *reinterpret_cast<u32x2_t*>(p.out + (first + h) * D + d) =
           u32x2_t{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
     } else {
-      const int64_t at = (first + h) * p.splits + split;
+      const int64_t at = (first + h) * splits + split;
       if (hl != 0.f) *reinterpret_cast<floatx4_t*>(p.part_o + at * D + d) = sum;
       if (d == 0) p.part_ml[2 * at] = hm, p.part_ml[2 * at + 1] = hl;
     }
   }
-  (void)total;
 }
 
-// out = sum of the splits' o 2^(m - M) over that of their l, times v_scale.
-// An empty split has l = 0 and its o is not there.
+// out = sum of the splits' o 2^(m - M) over that of their l, times v_scale.  An empty
+// split has l = 0, and its o is not there.
 constexpr int kMaxSplits = PD_BLOCK_SPLITS;
+constexpr int kFewSplits = 8;
 
-template <int D>
+// Up to kFewSplits (kMost of them at most): four columns a thread, every split in its
+// registers.
+template <int kMost>
 __global__ void __launch_bounds__(256)
-block_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                   const float* __restrict__ v_scale, uint16_t* __restrict__ out, int group,
-                   int heads, int splits) {
-  constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+few_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                 uint16_t* __restrict__ out, int splits, int dim, int64_t total,
+                 const float* __restrict__ v_scale, int group, int heads) {
+  const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (at >= total) return;
+  const int64_t bh = at / dim;
+  const int col = int(at - bh * dim);
+  floatx2_t ml[kMost];
+  floatx4_t o[kMost];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    const int64_t from = bh * splits + min(i, splits - 1);
+    ml[i] = *reinterpret_cast<const floatx2_t*>(part_ml + 2 * from);
+    o[i] = *reinterpret_cast<const floatx4_t*>(part_o + from * dim + col);
+    top = fmaxf(top, ml[i][0]);
+  }
+  const float base = top == -INFINITY ? 0.f : top;
+  floatx4_t sum = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    const bool real = i < splits && ml[i][1] != 0.f;
+    const float f = exp2_fast(ml[i][0] - base);
+    l += real ? f * ml[i][1] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += real ? f * o[i][e] : 0.f;
+  }
+  sum *= (v_scale ? v_scale[bh % heads / group] : 1.f) / (l == 0.f ? 1.f : l);
+  *reinterpret_cast<u32x2_t*>(out + at) =
+      u32x2_t{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
+}
+
+// More: 64 columns a workgroup, 16 rows of threads over the splits, kMost splits a thread.
+constexpr int kMergeCols = 64;
+
+template <int kMost>
+__global__ void __launch_bounds__(256)
+many_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                  uint16_t* __restrict__ out, int splits, int dim,
+                  const float* __restrict__ v_scale, int group, int heads) {
+  constexpr int kLanes = kMergeCols / 4, kRows = 256 / kLanes;
   __shared__ float weight[kMaxSplits];
   __shared__ float waves[4][2];
   __shared__ floatx4_t sums[kRows][kLanes];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t bh = blockIdx.x;
+  const int col = blockIdx.y * kMergeCols + 4 * (tid % kLanes), row = tid / kLanes;
+  const float* mine = part_o + bh * splits * dim + col;
+  // The rows are on their way while the weights are made.
+  floatx4_t o[kMost];
+#pragma unroll
+  for (int i = 0; i < kMost; ++i)
+    o[i] = *reinterpret_cast<const floatx4_t*>(mine +
+                                               int64_t(min(row + i * kRows, splits - 1)) * dim);
   float m = -INFINITY, l = 0.f;
   if (tid < splits) {
     m = part_ml[(bh * splits + tid) * 2];
@@ -583,22 +849,27 @@ block_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ p
   const float wl = wave_sum(l == 0.f ? 0.f : l * f);
   if (lane == 0) waves[w][1] = wl;
   __syncthreads();
-  const int part = tid % kLanes;
   floatx4_t sum = {0.f, 0.f, 0.f, 0.f};
-  for (int s = tid / kLanes; s < splits; s += kRows) {
-    const float x = weight[s];
-    if (!(x < 0.f))
-      sum += x * *reinterpret_cast<const floatx4_t*>(part_o + (bh * splits + s) * D + 4 * part);
-  }
-  sums[tid / kLanes][part] = sum;
-  __syncthreads();
-  if (tid >= kLanes) return;
 #pragma unroll
-  for (int r = 1; r < kRows; ++r) sum += sums[r][part];
+  for (int i = 0; i < kMost; ++i) {
+    const float x = row + i * kRows < splits ? weight[row + i * kRows] : -1.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += x < 0.f ? 0.f : x * o[i][e];
+  }
+  sums[row][tid % kLanes] = sum;
+  __syncthreads();
+  if (row) return;
+#pragma unroll
+  for (int r = 1; r < kRows; ++r) sum += sums[r][tid];
   const float total = waves[0][1] + waves[1][1] + waves[2][1] + waves[3][1];
   sum *= (v_scale ? v_scale[bh % heads / group] : 1.f) / (total == 0.f ? 1.f : total);
-  *reinterpret_cast<u32x2_t*>(out + bh * D + 4 * part) =
+  *reinterpret_cast<u32x2_t*>(out + bh * dim + col) =
       u32x2_t{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
+}
+
+int tile_tokens(int head_dim, int32_t cache_type) {
+  const int row = head_dim * (cache_type == PD_CACHE_E4M3 ? 1 : 2);
+  return row >= 512 ? 16 : row >= 256 ? 32 : 64;
 }
 
 int check_geometry(int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
@@ -611,8 +882,8 @@ int check_geometry(int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32
     return pd::fail(PD_EINVAL, "query heads must be divisible by KV heads");
   if (table_width < 1 || table_width >= 1 << 22)
     return pd::fail(PD_EINVAL, "table width must be in [1, 2^22)");
-  if (num_pages < 1 || num_pages > INT32_MAX)
-    return pd::fail(PD_EINVAL, "the page pool must hold at least one page");
+  if (num_pages < 1 || num_pages > 1 << 28)
+    return pd::fail(PD_EINVAL, "the page pool must hold 1 to 2^28 pages");
   if (int64_t(num_kv_heads) * head_dim * 512 > INT32_MAX)
     return pd::fail(PD_EINVAL, "a page of one KV tensor must be below 2 GiB");
   return PD_OK;
@@ -643,38 +914,65 @@ extern "C" int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_str
   p.blocks = blocks, p.qsb = q_stride_b, p.qsh = q_stride_h, p.tsb = table_stride_b;
   p.num_pages = num_pages, p.width = table_width, p.hkv = num_kv_heads;
   p.group = num_heads / num_kv_heads, p.kept = kept, p.first = first, p.last = last;
-  const int64_t most = int64_t(table_width) * kPerPage - first - last;
-  if (table_width * kPerPage > kept && most > 0) {
-    const auto go = [&](auto kernel, int per) {
-      hipLaunchKernelGGL(kernel, dim3(unsigned((most + per - 1) / per), num_kv_heads, batch),
-                         dim3(256), 0, as_stream(stream), p);
+  const int64_t wide = int64_t(table_width) * kPerPage;
+  if (wide > kept) {
+    const auto go = [&](auto dim, auto heads, auto whole) {
+      // Eight workgroups a CU at most: a wavefront then takes several runs with the query in
+      // its registers.  64 sequences of up to 32768 tokens, Hkv 8: 34.1 us with 1024
+      // workgroups, 27.9 with 2048, 28.9 with 4096 (both launches); 8 of up to 65536: 14.4,
+      // 15.7 and 16.8.
+      constexpr int kPer = 4 * Scores<dim.value>::kPer;
+      const int64_t groups = (wide + kPer - 1) / kPer;
+      const int64_t most = std::max<int64_t>(1, 2048 / (int64_t(batch) * num_kv_heads));
+      hipLaunchKernelGGL((score_kernel<dim.value, heads.value, whole.value>),
+                         dim3(unsigned(std::min(groups, most)), num_kv_heads, batch), dim3(256), 0,
+                         as_stream(stream), p);
+    };
+    const auto with = [&](auto dim) {
+      if (p.group == 1)
+        go(dim, std::integral_constant<int, 1>{}, std::true_type{});
+      else if (p.group == 2)
+        go(dim, std::integral_constant<int, 2>{}, std::true_type{});
+      else if (p.group <= 4)
+        go(dim, std::integral_constant<int, 4>{}, std::true_type{});
+      else
+        go(dim, std::integral_constant<int, 4>{}, std::false_type{});
     };
     if (head_dim == 64)
-      go(score_kernel<64>, Scores<64>::kBlocks);
+      with(std::integral_constant<int, 64>{});
     else if (head_dim == 128)
-      go(score_kernel<128>, Scores<128>::kBlocks);
+      with(std::integral_constant<int, 128>{});
     else
-      go(score_kernel<256>, Scores<256>::kBlocks);
+      with(std::integral_constant<int, 256>{});
     if (const int bad = launch_status("pd_select_blocks")) return bad;
   }
-  hipLaunchKernelGGL(pick_kernel, dim3(num_kv_heads, batch), dim3(256), 0, as_stream(stream), p);
+  hipLaunchKernelGGL(pick_kernel, dim3(num_kv_heads, batch), dim3(64 * kPickWaves), 0,
+                     as_stream(stream), p);
   return launch_status("pd_select_blocks");
 }
 
 extern "C" int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_heads,
-                               int32_t entries, int32_t cus, int32_t* splits) {
+                               int32_t head_dim, int32_t cache_type, int32_t entries,
+                               int32_t listed, int32_t cus, int32_t* splits) {
   pd::clear_error();
   if (batch < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || num_heads % num_kv_heads ||
       entries < 1 || cus < 1 || !splits)
     return pd::fail(PD_EINVAL, "batch, heads, entries and CUs must be positive");
+  if (!pd::valid_head_dim(head_dim) || !pd::valid_cache(cache_type))
+    return pd::fail(PD_EINVAL, "unknown head_dim or cache type");
   int64_t rows = 1;
   while (rows < batch) rows *= 2;
   rows *= int64_t(num_kv_heads) * ((num_heads / num_kv_heads + 15) / 16);
-  const int64_t want = (8 * int64_t(cus) + rows - 1) / rows;
-  const int64_t most = (int64_t(entries) + 3) / 4;
-  int64_t s = want < most ? want : most;
-  if (s > kMaxSplits) s = kMaxSplits;
-  *splits = int32_t(s < 1 ? 1 : s);
+  // Listed blocks are as many for every row: one workgroup a CU, each with the most to do
+  // behind its start of some 3 us (17 rows of 37 blocks, Hq 32 / Hkv 4 / D 256, e4m3: 23.5 us;
+  // 26.9 with two, 30.2 with eight).  Whole caches differ in length: eight a CU, so that no
+  // long one is left to a few (64 of 1 to 32768 tokens, Hq 32 / Hkv 8 / D 128: 394 us; 604 with
+  // two; 8 of 1000 to 9000: 26.3 and 25.1).
+  const int64_t groups = int64_t(listed ? 1 : 8) * cus;
+  const int64_t want = (groups + rows - 1) / rows;
+  const int64_t tiles = int64_t(entries) * (kBlock / tile_tokens(head_dim, cache_type));
+  const int64_t most = std::min<int64_t>((tiles + 3) / 4, kMaxSplits);
+  *splits = int32_t(std::max<int64_t>(1, std::min(want, most)));
   return PD_OK;
 }
 
@@ -692,39 +990,49 @@ extern "C" int pd_block_decode(const void* q, int64_t q_stride_b, int64_t q_stri
           check_geometry(batch, num_heads, num_kv_heads, head_dim, table_width, num_pages))
     return bad;
   if (!pd::valid_cache(cache_type)) return pd::fail(PD_EINVAL, "unknown cache type");
-  if (blocks && kept < 1) return pd::fail(PD_EINVAL, "the list must hold at least one block");
+  if (blocks && (kept < 1 || kept > 1 << 26))
+    return pd::fail(PD_EINVAL, "the list must hold at least one block, at most 2^26");
   if (splits < 1 || splits > kMaxSplits)
     return pd::fail(PD_EINVAL, "splits must be in [1, %d]", kMaxSplits);
   if (!q || !k || !v || !table || !lengths || !out || (splits > 1 && (!part_o || !part_ml)) ||
-      !all_aligned16(q, k, v, part_o, out) || q_stride_b % 8 || q_stride_h % 8)
+      !all_aligned16(q, k, v, part_o, part_ml, out) || q_stride_b % 8 || q_stride_h % 8)
     return pd::fail(PD_EINVAL, "tensors must be present, with 16-byte aligned rows");
   DecodeArgs p;
-  p.q = u16(q), p.k = static_cast<const char*>(k), p.v = static_cast<const char*>(v);
-  p.table = table, p.lengths = lengths, p.blocks = blocks, p.k_scale = k_scale;
-  p.v_scale = v_scale, p.part_o = part_o, p.part_ml = part_ml, p.out = u16(out);
-  p.qsb = q_stride_b, p.qsh = q_stride_h, p.tsb = table_stride_b, p.num_pages = num_pages;
-  p.width = table_width, p.hkv = num_kv_heads, p.group = num_heads / num_kv_heads;
-  p.tiles = (p.group + 15) / 16, p.kept = kept, p.splits = splits;
+  p.k_scale = k_scale, p.v_scale = v_scale, p.part_o = part_o, p.part_ml = part_ml;
+  p.out = u16(out), p.qsb = q_stride_b, p.qsh = q_stride_h;
+  p.group = num_heads / num_kv_heads, p.tiles = (p.group + 15) / 16;
   p.scale2 = float(scale * 1.4426950408889634);
-  const int64_t groups = int64_t(batch) * splits * num_kv_heads * p.tiles;
-  if (groups > 0x7fffffff || int64_t(batch) * num_heads > 0x7fffffff)
+  const int64_t columns = int64_t(num_kv_heads) * p.tiles;
+  if (batch > 65535 || columns * splits * batch > 0x7fffffff)
     return pd::fail(PD_EINVAL, "grid dimension exceeds device limits");
+  const dim3 grid = {unsigned(columns), unsigned(splits), unsigned(batch)};
   const unsigned lds = unsigned(128 + 4 * (p.group < 16 ? p.group : 16) * head_dim) * 4;
   pd::for_cache(head_dim, cache_type, [&](auto dim, auto e4m3) {
-    hipLaunchKernelGGL((block_decode_kernel<dim.value, e4m3.value>), dim3(unsigned(groups)),
-                       dim3(256), lds, as_stream(stream), p);
+    hipLaunchKernelGGL((block_decode_kernel<dim.value, e4m3.value>), grid, dim3(256), lds,
+                       as_stream(stream), lengths, blocks, table, table_stride_b, table_width,
+                       kept, num_kv_heads, int(num_pages), static_cast<const char*>(k),
+                       static_cast<const char*>(v), u16(q), p);
   });
   if (const int bad = launch_status("pd_block_decode")) return bad;
   if (splits == 1) return PD_OK;
-  const auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(unsigned(batch * num_heads)), dim3(256), 0, as_stream(stream),
-                       part_o, part_ml, v_scale, p.out, p.group, num_heads, splits);
-  };
-  if (head_dim == 64)
-    merge(block_merge_kernel<64>);
-  else if (head_dim == 128)
-    merge(block_merge_kernel<128>);
-  else
-    merge(block_merge_kernel<256>);
-  return launch_status("pd_block_decode merge");
+  if (splits <= kFewSplits) {
+    const int64_t total = int64_t(batch) * num_heads * head_dim;
+    const auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(unsigned((total + 1023) / 1024)), dim3(256), 0,
+                         as_stream(stream), part_o, part_ml, p.out, splits, head_dim, total,
+                         v_scale, p.group, num_heads);
+    };
+    go(splits <= 2 ? few_merge_kernel<2> : splits <= 4 ? few_merge_kernel<4> : few_merge_kernel<8>);
+  } else {
+    const auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(unsigned(batch * num_heads), head_dim / kMergeCols),
+                         dim3(256), 0, as_stream(stream), part_o, part_ml, p.out, splits, head_dim,
+                         v_scale, p.group, num_heads);
+    };
+    go(splits <= 16   ? many_merge_kernel<1>
+       : splits <= 32 ? many_merge_kernel<2>
+       : splits <= 64 ? many_merge_kernel<4>
+                      : many_merge_kernel<8>);
+  }
+  return launch_status("pd_block_decode");
 }

@@ -81,7 +81,7 @@ SIGNATURES = {
     "pd_block_bounds": [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _i32, _vp],
     "pd_select_blocks": [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32,
                          _i32, _i32, _i32, _i32, _vp],
-    "pd_block_splits": [_i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i32)],
+    "pd_block_splits": [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, ctypes.POINTER(_i32)],
     "pd_block_decode": [_vp, _i64, _i64, _vp, _vp, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _i32, _vp,
                         _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _dbl, _vp],
 }
@@ -436,63 +436,30 @@ def delta_step(act, a, b, a_log, dt_bias, z, norm, eps, state, out, batch, hk, h
                               int(has_prev), stream_handle(act.device)))
 
 
-def on_device(index, launch, *args):
-    """``launch(*args)`` with tensors of CUDA device ``index``: the default stream's handle is
-    the same on every device and means the current one's."""
-    if torch.cuda.current_device() == index:
-        check(launch(*args, stream_handle(torch.device("cuda", index))))
-    else:
+# The current device without torch.cuda's lazy-initialization check: a caller holds a CUDA
+# tensor.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(index, function, *args):
+    """``function(*args, stream)`` for tensors of CUDA device ``index``, on its current stream.
+    The default stream's handle is the same on every device and means the current one's."""
+    if _current_device() != index:
         with torch.cuda.device(index):
-            check(launch(*args, stream_handle(torch.device("cuda", index))))
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+            check(function(*args, stream_handle(torch.device("cuda", index))))
+        return
+    status = function(*args, _raw_stream(index) if _raw_stream is not None
+                      else stream_handle(torch.device("cuda", index)))
+    if status:
+        check(status)
 
 
 CACHE_TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1}
 BLOCK, MAX_BLOCK_SPLITS = 64, 128
 
 
-def append_kv(q, k, v, positions, rope, interleaved, q_out, k_cache, v_cache, slot_mapping, k_scale,
-              v_scale, bounds):
-    """q and q_out [N, Hq, D] or None; k, v [N, Hkv, D]; rope [M, half, 2] or None."""
-    n, hkv, d = k.shape
-    on_device(k.get_device(), lib().pd_append_kv, _ptr(q), 0 if q is None else q.stride(0),
-              k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), _ptr(positions), _ptr(rope),
-              0 if rope is None else rope.shape[0], 0 if rope is None else rope.shape[1],
-              interleaved, _ptr(q_out), 0 if q is None else q_out.stride(0), k_cache.data_ptr(),
-              v_cache.data_ptr(), CACHE_TYPES[k_cache.dtype], k_cache.shape[0] * k_cache.shape[1],
-              slot_mapping.data_ptr(), _ptr(k_scale), _ptr(v_scale), _ptr(bounds), n,
-              0 if q is None else q.shape[1], hkv, d)
-
-
-def block_bounds(k_cache, slot_mapping, bounds):
-    on_device(k_cache.get_device(), lib().pd_block_bounds, k_cache.data_ptr(),
-              CACHE_TYPES[k_cache.dtype], k_cache.shape[0] * k_cache.shape[1],
-              slot_mapping.data_ptr(), slot_mapping.shape[0], bounds.data_ptr(), k_cache.shape[2],
-              k_cache.shape[3])
-
-
-def select_blocks(q, bounds, tables, lengths, keys, blocks, num_kv_heads, first, last):
-    b, h, d = q.shape
-    on_device(q.get_device(), lib().pd_select_blocks, q.data_ptr(), q.stride(0), q.stride(1),
-              bounds.data_ptr(), bounds.shape[0], tables.data_ptr(), tables.stride(0),
-              tables.shape[1], lengths.data_ptr(), keys.data_ptr(), blocks.data_ptr(),
-              blocks.shape[2], first, last, b, h, num_kv_heads, d)
-
-
-def block_splits(batch, num_heads, num_kv_heads, entries, cus):
+def block_splits(batch, num_heads, num_kv_heads, head_dim, dtype, entries, listed, cus):
     splits = _i32(0)
-    check(lib().pd_block_splits(batch, num_heads, num_kv_heads, entries, cus, ctypes.byref(splits)))
+    check(lib().pd_block_splits(batch, num_heads, num_kv_heads, head_dim, CACHE_TYPES[dtype], entries,
+                                int(listed), cus, ctypes.byref(splits)))
     return splits.value
-
-
-def block_decode(q, k, v, tables, lengths, blocks, k_scale, v_scale, part_o, part_ml, splits, out,
-                 num_kv_heads, scale):
-    b, h, d = q.shape
-    on_device(q.get_device(), lib().pd_block_decode, q.data_ptr(), q.stride(0), q.stride(1),
-              k.data_ptr(), v.data_ptr(), CACHE_TYPES[k.dtype], k.shape[0], tables.data_ptr(),
-              tables.stride(0), tables.shape[1], lengths.data_ptr(), _ptr(blocks),
-              0 if blocks is None else blocks.shape[2], _ptr(k_scale), _ptr(v_scale), _ptr(part_o),
-              _ptr(part_ml), splits, out.data_ptr(), b, h, num_kv_heads, d, scale)

@@ -39,13 +39,13 @@ class BlockResources:
     sm_count: int = 0
     _splits: dict = field(default_factory=dict, repr=False, compare=False)
 
-    def splits(self, batch):
-        found = self._splits.get(batch)
+    def splits(self, batch, dtype):
+        found = self._splits.get((batch, dtype))
         if found is None:
             spec = self.spec
-            found = self._splits[batch] = _native.block_splits(
-                batch, spec.num_heads, spec.num_kv_heads,
-                self.kept or spec.table_width * _PER_PAGE, self.sm_count)
+            found = self._splits[batch, dtype] = _native.block_splits(
+                batch, spec.num_heads, spec.num_kv_heads, spec.head_dim, dtype,
+                self.kept or spec.table_width * _PER_PAGE, self.kept > 0, self.sm_count)
         return found
 
 
@@ -64,7 +64,7 @@ def allocate_block_resources(spec, device, *, kept=0):
     rows, batch = 0, 1
     while batch < 2 * spec.max_batch:
         batch = min(batch, spec.max_batch)
-        splits = result.splits(batch)
+        splits = max(result.splits(batch, dtype) for dtype in _native.CACHE_TYPES)
         rows = max(rows, batch * heads * splits if splits > 1 else 0)
         batch *= 2
     result.partials, result.sums = make(rows * dim), make(rows * 2)
@@ -75,48 +75,60 @@ def allocate_block_resources(spec, device, *, kept=0):
 
 
 def _check_step(q, tables, lengths, resources):
-    spec = resources.spec
+    """(batch, device, Q's strides, the table's row stride and width)."""
+    spec, shape, stride = resources.spec, q.shape, q.stride()
     device = q.get_device()
     if device < 0 or not (tables.get_device() == lengths.get_device()
                           == resources.out.get_device() == device):
         raise ValueError("all tensors must be on the same CUDA device")
     if q.dtype != torch.bfloat16:
         raise ValueError("BF16 Q required")
-    if q.ndim != 3 or q.shape[1:] != (spec.num_heads, spec.head_dim):
+    if len(shape) != 3 or shape[1] != spec.num_heads or shape[2] != spec.head_dim:
         raise ValueError("Q must have shape [batch, query_heads, head_dim]")
-    batch = q.shape[0]
-    if not 0 < batch <= spec.max_batch or q.stride(2) != 1:
+    batch = shape[0]
+    if not 0 < batch <= spec.max_batch or stride[2] != 1:
         raise ValueError("Q batch exceeds capacity or innermost dimension is not contiguous")
-    if tables.ndim != 2 or tables.shape[0] != batch or tables.stride(1) != 1:
+    form, step = tables.shape, tables.stride()
+    if len(form) != 2 or form[0] != batch or step[1] != 1:
         raise ValueError("block table must have shape [batch,capacity] and contiguous rows")
-    if not 0 < tables.shape[1] <= spec.table_width:
+    if not 0 < form[1] <= spec.table_width:
         raise ValueError("block table width outside configured capacity")
     if lengths.shape != (batch,) or not lengths.is_contiguous():
         raise ValueError("context lengths must be a contiguous [batch] tensor")
     if tables.dtype != torch.int32 or lengths.dtype != torch.int32:
         raise ValueError("block tables and context lengths must be int32")
-    return batch, device
+    return batch, device, stride[0], stride[1], step[0], form[1]
 
 
 def _attend(q, k, v, tables, lengths, blocks, resources, scale, k_scale, v_scale):
-    batch, device = _check_step(q, tables, lengths, resources)
-    spec = resources.spec
-    if k.dtype not in _native.CACHE_TYPES or v.dtype != k.dtype:
-        raise ValueError("caches must be BF16 or float8_e4m3fn")
-    if k.ndim != 4 or k.shape[1:] != (256, spec.num_kv_heads, spec.head_dim):
+    batch, device, stride_b, stride_h, table_stride, width = _check_step(q, tables, lengths,
+                                                                         resources)
+    spec, shape, kind = resources.spec, k.shape, k.dtype
+    cache_type = _native.CACHE_TYPES.get(kind)
+    if cache_type is None or v.dtype != kind:
+        raise ValueError("caches must both be BF16 or float8_e4m3fn")
+    hkv, dim = spec.num_kv_heads, spec.head_dim
+    if len(shape) != 4 or shape[1] != 256 or shape[2] != hkv or shape[3] != dim:
         raise ValueError("KV must use NHD pages [pages,256,kv_heads,head_dim]")
-    if k.shape != v.shape or not k.is_contiguous() or not v.is_contiguous() or k.shape[0] == 0:
+    if v.shape != shape or not k.is_contiguous() or not v.is_contiguous() or shape[0] == 0:
         raise ValueError("K/V must have matching nonempty contiguous storage")
     if k.get_device() != device or v.get_device() != device:
         raise ValueError("all tensors must be on the same CUDA device")
-    check_scales(k_scale, v_scale, k.dtype, spec.num_kv_heads, device)
-    scale = spec.head_dim ** -0.5 if scale is None else float(scale)
+    if k_scale is not None or v_scale is not None:
+        check_scales(k_scale, v_scale, kind, hkv, device)
+    scale = dim ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
-    splits = resources.splits(batch)
-    _native.block_decode(q, k, v, tables, lengths, blocks, k_scale, v_scale, resources.partials,
-                         resources.sums, splits, resources.out, spec.num_kv_heads, scale)
-    return resources.out if batch == spec.max_batch else resources.out[:batch]
+    out = resources.out
+    _native.launch(device, _native.lib().pd_block_decode, q.data_ptr(), stride_b, stride_h,
+                   k.data_ptr(), v.data_ptr(), cache_type, shape[0], tables.data_ptr(), table_stride,
+                   width, lengths.data_ptr(), None if blocks is None else blocks.data_ptr(),
+                   0 if blocks is None else blocks.shape[2],
+                   None if k_scale is None else k_scale.data_ptr(),
+                   None if v_scale is None else v_scale.data_ptr(), resources.partials.data_ptr(),
+                   resources.sums.data_ptr(), resources.splits(batch, kind), out.data_ptr(), batch,
+                   spec.num_heads, hkv, dim, scale)
+    return out if batch == spec.max_batch else out[:batch]
 
 
 def fp8_decode(q, k, v, tables, lengths, *, resources, scale=None, k_scale=None, v_scale=None):
@@ -140,17 +152,20 @@ def select_blocks(q, bounds, tables, lengths, *, resources, first=1, last=1):
     ``bounds`` as of ``kv_append``, of the keys as they are stored (a scale per kv head moves
     no block).  ``last`` is at least 1: the block being filled has no bounds.  A NaN score
     counts as infinite."""
-    batch, device = _check_step(q, tables, lengths, resources)
-    spec = resources.spec
+    batch, device, stride_b, stride_h, table_stride, width = _check_step(q, tables, lengths,
+                                                                         resources)
+    spec, blocks = resources.spec, resources.blocks
     if not resources.kept:
         raise ValueError("these resources hold no list of blocks: allocate them with kept=")
-    if (bounds.shape[1:] != (_PER_PAGE, spec.num_kv_heads, 2, spec.head_dim)
-            or bounds.dtype != torch.bfloat16 or not bounds.is_contiguous()
-            or bounds.get_device() != device or bounds.shape[0] == 0):
+    hkv, dim, shape = spec.num_kv_heads, spec.head_dim, bounds.shape
+    if (shape[1:] != (_PER_PAGE, hkv, 2, dim) or bounds.dtype != torch.bfloat16
+            or not bounds.is_contiguous() or bounds.get_device() != device or shape[0] == 0):
         raise ValueError("bounds must be contiguous BF16 [pages, 4, kv_heads, 2, head_dim]")
-    _native.select_blocks(q, bounds, tables, lengths, resources.keys, resources.blocks,
-                          spec.num_kv_heads, first, last)
-    return resources.blocks if batch == spec.max_batch else resources.blocks[:batch]
+    _native.launch(device, _native.lib().pd_select_blocks, q.data_ptr(), stride_b, stride_h,
+                   bounds.data_ptr(), shape[0], tables.data_ptr(), table_stride, width,
+                   lengths.data_ptr(), resources.keys.data_ptr(), blocks.data_ptr(), resources.kept,
+                   first, last, batch, spec.num_heads, hkv, dim)
+    return blocks if batch == spec.max_batch else blocks[:batch]
 
 
 def sparse_decode(q, k, v, tables, lengths, blocks, *, resources, scale=None, k_scale=None,
@@ -161,8 +176,9 @@ def sparse_decode(q, k, v, tables, lengths, blocks, *, resources, scale=None, k_
     the length have no tokens, an entry listed twice counts twice, no token gives zeros."""
     if not resources.kept:
         raise ValueError("these resources hold no list of blocks: allocate them with kept=")
-    if (blocks.ndim != 3 or blocks.shape[:2] != (q.shape[0], resources.spec.num_kv_heads)
-            or not 0 < blocks.shape[2] <= resources.kept or blocks.dtype != torch.int32
+    form = blocks.shape
+    if (len(form) != 3 or form[0] != q.shape[0] or form[1] != resources.spec.num_kv_heads
+            or not 0 < form[2] <= resources.kept or blocks.dtype != torch.int32
             or not blocks.is_contiguous() or blocks.get_device() != q.get_device()):
         raise ValueError("blocks must be contiguous int32 [batch, kv_heads, listed], at most kept")
     return _attend(q, k, v, tables, lengths, blocks, resources, scale, k_scale, v_scale)

@@ -17,7 +17,6 @@ hipGraph.  Inference only.
 import torch
 
 from . import _native
-from .kv_write import _require
 
 BLOCK = _native.BLOCK
 
@@ -26,8 +25,8 @@ def rope_cache(max_positions, inv_freq, device="cuda"):
     """float32 [max_positions, half, 2]: (cos, sin) of position x inv_freq [half], the angles
     in float64 (a float32 angle is off by 0.004 at position 65536)."""
     inv = torch.as_tensor(inv_freq, dtype=torch.float64, device=device)
-    _require(inv.dim() == 1 and type(max_positions) is int and max_positions > 0,
-             "rope_cache needs positions and inv_freq [half]")
+    if inv.dim() != 1 or type(max_positions) is not int or max_positions < 1:
+        raise ValueError("rope_cache needs positions and inv_freq [half]")
     angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * inv
     return torch.stack([angle.cos(), angle.sin()], -1).float()
 
@@ -35,54 +34,66 @@ def rope_cache(max_positions, inv_freq, device="cuda"):
 def allocate_bounds(k_cache):
     """bf16 [pages, page_size // 64, Hkv, 2, D] (smallest, largest) for a key cache, zeros."""
     pages, size, hkv, dim = k_cache.shape
-    _require(size % BLOCK == 0, "bounds need pages of whole blocks of 64 slots")
+    if size % BLOCK:
+        raise ValueError("bounds need pages of whole blocks of 64 slots")
     return torch.zeros((pages, size // BLOCK, hkv, 2, dim), dtype=torch.bfloat16,
                        device=k_cache.device)
 
 
-def _check_cache(k_cache, bounds, device):
-    _require(k_cache.dim() == 4 and k_cache.is_contiguous(),
-             "caches must be contiguous [blocks, block_size, kv_heads, head_dim]")
-    _require(k_cache.dtype in _native.CACHE_TYPES, "caches must be BF16 or float8_e4m3fn")
-    if bounds is not None:
-        pages, size, hkv, dim = k_cache.shape
-        _require(size % BLOCK == 0 and bounds.shape == (pages, size // BLOCK, hkv, 2, dim)
-                 and bounds.dtype == torch.bfloat16 and bounds.is_contiguous()
-                 and bounds.get_device() == device,
-                 "bounds must be contiguous BF16 [pages, page_size // 64, kv_heads, 2, head_dim] "
-                 "on the cache's device")
+def _refuse(message):
+    raise ValueError(message)
 
 
-def _check_rows(t, n, dim, device, what):
-    _require(t.dim() == 3 and t.shape[0] == n and t.shape[2] == dim,
-             f"{what} must be [N, heads, head_dim]")
-    _require(t.dtype == torch.bfloat16, "BF16 query/key/value required")
-    _require(t.stride(2) == 1 and (t.stride(1) == dim or t.shape[1] == 1),
-             f"{what} heads must be contiguous")
-    _require(t.get_device() == device, "all tensors must be on one CUDA device")
+def _pointer(t):
+    return None if t is None else t.data_ptr()
+
+
+def _row_stride(t, rows, heads, dim, device, what):
+    """Elements between the rows of t [rows, heads or any number (None), dim]."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] != rows or shape[2] != dim or heads not in (None, shape[1]):
+        _refuse(f"{what} must be [N, heads, head_dim] with the key's rows")
+    if t.dtype != torch.bfloat16:
+        _refuse("BF16 query/key/value required")
+    if stride[2] != 1 or (stride[1] != dim and shape[1] != 1):
+        _refuse(f"{what} heads must be contiguous")
+    if t.get_device() != device:
+        _refuse("all tensors must be on one CUDA device")
+    return stride[0]
 
 
 def _check_index(t, n, dtype, device, what):
-    _require(t.dim() == 1 and t.shape[0] == n and t.dtype == dtype and t.is_contiguous(),
-             f"{what} must be contiguous {str(dtype)[6:]} with one entry per token")
-    _require(t.get_device() == device, "all tensors must be on one CUDA device")
+    if t.shape != (n,) or t.dtype != dtype or not t.is_contiguous() or t.get_device() != device:
+        _refuse(f"{what} must be contiguous {str(dtype)[6:]} with one entry per token, on the "
+                "cache's device")
+
+
+def _check_bounds(bounds, cache_shape, device):
+    pages, size, hkv, dim = cache_shape
+    if (size % BLOCK or bounds.shape != (pages, size // BLOCK, hkv, 2, dim)
+            or bounds.dtype != torch.bfloat16 or not bounds.is_contiguous()
+            or bounds.get_device() != device):
+        _refuse("bounds must be contiguous BF16 [pages, page_size // 64, kv_heads, 2, head_dim] "
+                "on the cache's device")
 
 
 def check_scales(k_scale, v_scale, dtype, hkv, device):
     for t in (k_scale, v_scale):
-        if t is not None:
-            _require(dtype == torch.float8_e4m3fn, "scales belong to a float8_e4m3fn cache")
-            _require(t.shape == (hkv,) and t.dtype == torch.float32 and t.is_contiguous()
-                     and t.get_device() == device,
-                     "scales must be contiguous float32 [kv_heads] on the cache's device")
+        if t is None:
+            continue
+        if dtype != torch.float8_e4m3fn:
+            _refuse("scales belong to a float8_e4m3fn cache")
+        if (t.shape != (hkv,) or t.dtype != torch.float32 or not t.is_contiguous()
+                or t.get_device() != device):
+            _refuse("scales must be contiguous float32 [kv_heads] on the cache's device")
 
 
 def append_kv(q, k, v, positions, rope, k_cache, v_cache, slot_mapping, *, interleaved=False,
               k_scale=None, v_scale=None, bounds=None, out=None):
     """Rotated queries [N, Hq, D]; keys (rotated) and values written to their slots.
 
-    q [N, Hq, D] (or None: returns None), k and v [N, Hkv, D] bf16, heads contiguous; rows may be slices of a
-    fused projection.  ``rope`` float32 [M, half, 2] (``rope_cache``) and ``positions`` int64
+    q [N, Hq, D] (or None: returns None), k and v [N, Hkv, D] bf16, heads contiguous; rows may
+    be slices of a fused projection.  ``rope`` float32 [M, half, 2] (``rope_cache``) and ``positions`` int64
     [N]: element pairs (j, j + half), or (2j, 2j + 1) with ``interleaved``, of the leading
     2 half elements are rotated, half a multiple of 8; rope None rotates nothing.
     Caches [blocks, block_size, Hkv, D] bf16 or float8_e4m3fn, which holds x / scale, clamped
@@ -90,48 +101,68 @@ def append_kv(q, k, v, positions, rope, k_cache, v_cache, slot_mapping, *, inter
     nothing, slots of one call must differ.  A position outside the table writes nothing and
     gives its query NaN.  ``out``: where the queries go (q itself: in place).
     """
-    _require(k.dim() == 3 and k.is_cuda, "key must be [N, kv_heads, head_dim] on a CUDA device")
-    n, hkv, dim = k.shape
-    device = k.get_device()
-    _check_rows(k, n, dim, device, "key")
-    _check_rows(v, n, dim, device, "value")
-    _require(v.shape == k.shape, "value must have the key's shape")
-    _check_cache(k_cache, bounds, device)
-    _require(v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype
-             and v_cache.is_contiguous() and k_cache.shape[2:] == (hkv, dim),
-             "caches must have one shape and type, and the key's heads")
-    _require(k_cache.get_device() == device and v_cache.get_device() == device,
-             "all tensors must be on one CUDA device")
+    shape, device = k.shape, k.get_device()
+    if len(shape) != 3 or device < 0:
+        _refuse("key must be [N, kv_heads, head_dim] on a CUDA device")
+    n, hkv, dim = shape
+    k_stride = _row_stride(k, n, hkv, dim, device, "key")
+    v_stride = _row_stride(v, n, hkv, dim, device, "value")
+    cache, kind = k_cache.shape, k_cache.dtype
+    cache_type = _native.CACHE_TYPES.get(kind)
+    if cache_type is None or v_cache.dtype != kind:
+        _refuse("caches must both be BF16 or float8_e4m3fn")
+    if (len(cache) != 4 or cache[2] != hkv or cache[3] != dim or v_cache.shape != cache
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+        _refuse("caches must be contiguous [blocks, block_size, kv_heads, head_dim] with the "
+                "key's heads")
+    if k_cache.get_device() != device or v_cache.get_device() != device:
+        _refuse("all tensors must be on one CUDA device")
     _check_index(slot_mapping, n, torch.int32, device, "slot_mapping")
-    check_scales(k_scale, v_scale, k_cache.dtype, hkv, device)
+    if k_scale is not None or v_scale is not None:
+        check_scales(k_scale, v_scale, kind, hkv, device)
+    if bounds is not None:
+        _check_bounds(bounds, cache, device)
+    table = (None, None, 0, 0)
     if rope is not None:
-        _require(rope.dim() == 3 and rope.shape[2] == 2 and rope.dtype == torch.float32
-                 and rope.is_contiguous() and rope.get_device() == device,
-                 "rope must be contiguous float32 [positions, half, 2] on the key's device")
+        form = rope.shape
+        if (len(form) != 3 or form[2] != 2 or rope.dtype != torch.float32
+                or not rope.is_contiguous() or rope.get_device() != device):
+            _refuse("rope must be contiguous float32 [positions, half, 2] on the key's device")
         _check_index(positions, n, torch.int64, device, "positions")
+        table = (positions.data_ptr(), rope.data_ptr(), form[0], form[1])
+    heads = q_stride = out_stride = 0
     if q is not None:
-        _check_rows(q, n, dim, device, "query")
+        q_stride, heads = _row_stride(q, n, None, dim, device, "query"), q.shape[1]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out_stride = heads * dim
         else:
-            _require(out.shape == q.shape, "out must have the query's shape")
-            _check_rows(out, n, dim, device, "out")
-    else:
-        _require(out is None, "out needs a query")
+            out_stride = _row_stride(out, n, heads, dim, device, "out")
+    elif out is not None:
+        _refuse("out needs a query")
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad
                                     or (q is not None and q.requires_grad)):
-        raise ValueError("append_kv has no gradient: call it under torch.no_grad()")
-    _native.append_kv(q, k, v, positions if rope is not None else None, rope, interleaved, out,
-                      k_cache, v_cache, slot_mapping, k_scale, v_scale, bounds)
+        _refuse("append_kv has no gradient: call it under torch.no_grad()")
+    _native.launch(device, _native.lib().pd_append_kv, _pointer(q), q_stride, k.data_ptr(), k_stride,
+                   v.data_ptr(), v_stride, *table, interleaved, _pointer(out), out_stride,
+                   k_cache.data_ptr(), v_cache.data_ptr(), cache_type, cache[0] * cache[1],
+                   slot_mapping.data_ptr(), _pointer(k_scale), _pointer(v_scale), _pointer(bounds),
+                   n, heads, hkv, dim)
     return out
 
 
 def block_bounds(k_cache, slot_mapping, bounds):
     """Sets the bounds of every block whose last slot is in ``slot_mapping`` (int32 [N]) from
     the keys in the cache: for blocks that ``append_kv`` did not write."""
-    _require(k_cache.is_cuda, "the cache must be on a CUDA device")
-    device = k_cache.get_device()
-    _check_cache(k_cache, bounds, device)
-    _require(bounds is not None and slot_mapping.dim() == 1, "bounds and slots are required")
-    _check_index(slot_mapping, slot_mapping.shape[0], torch.int32, device, "slot_mapping")
-    _native.block_bounds(k_cache, slot_mapping, bounds)
+    shape, device = k_cache.shape, k_cache.get_device()
+    if len(shape) != 4 or device < 0 or not k_cache.is_contiguous():
+        _refuse("the cache must be contiguous [blocks, block_size, kv_heads, head_dim] on a CUDA "
+                "device")
+    if k_cache.dtype not in _native.CACHE_TYPES:
+        _refuse("caches must be BF16 or float8_e4m3fn")
+    _check_bounds(bounds, shape, device)
+    n = slot_mapping.numel()
+    _check_index(slot_mapping, n, torch.int32, device, "slot_mapping")
+    _native.launch(device, _native.lib().pd_block_bounds, k_cache.data_ptr(),
+                   _native.CACHE_TYPES[k_cache.dtype], shape[0] * shape[1], slot_mapping.data_ptr(),
+                   n, bounds.data_ptr(), shape[2], shape[3])

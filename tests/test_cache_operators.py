@@ -1,6 +1,5 @@
 """Host side of the cache operators without a GPU: refusals before any launch, plans, and the
 64-bit forms on small cases worked out by hand."""
-import ctypes
 import math
 
 import pytest
@@ -76,17 +75,22 @@ def test_decode_arguments(change, message):
     assert message in _native.lib().pd_last_error()
 
 
-def test_splits():
+@pytest.mark.parametrize("dtype", [BF16, torch.float8_e4m3fn], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_splits(dim, dtype):
     for batch, heads, hkv, entries in ((1, 16, 4, 33), (128, 16, 16, 64), (64, 32, 8, 512),
                                        (3, 40, 2, 100000), (65535, 8, 8, 1)):
-        s = _native.block_splits(batch, heads, hkv, entries, 256)
-        assert 1 <= s <= min(_native.MAX_BLOCK_SPLITS, -(-entries // 4))
-        bucket = 1 << (batch - 1).bit_length()
-        assert s == _native.block_splits(bucket, heads, hkv, entries, 256)
+        for listed in (False, True):
+            s = _native.block_splits(batch, heads, hkv, dim, dtype, entries, listed, 256)
+            assert 1 <= s <= min(_native.MAX_BLOCK_SPLITS, entries)
+            bucket = 1 << (batch - 1).bit_length()
+            assert s == _native.block_splits(bucket, heads, hkv, dim, dtype, entries, listed, 256)
     with pytest.raises(ValueError, match="positive"):
-        _native.block_splits(0, 8, 2, 4, 256)
-    found = ctypes.c_int32(0)
-    assert _native.lib().pd_block_splits(1, 9, 2, 4, 256, ctypes.byref(found)) == _native.PD_EINVAL
+        _native.block_splits(0, 8, 2, dim, dtype, 4, False, 256)
+    with pytest.raises(ValueError, match="positive"):
+        _native.block_splits(1, 9, 2, dim, dtype, 4, False, 256)
+    with pytest.raises(ValueError, match="head_dim"):
+        _native.block_splits(1, 8, 2, 80, dtype, 4, False, 256)
 
 
 def test_rotation_table_holds_far_positions():

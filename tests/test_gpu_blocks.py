@@ -8,7 +8,6 @@ if not torch.cuda.is_available():
     pytest.skip("needs an MI355X GPU", allow_module_level=True)
 
 from oracle import blocks as O
-from paged_decode import _native
 from paged_decode.block_decode import (allocate_block_resources, fp8_decode, select_blocks,
                                        sparse_decode)
 from paged_decode.kv_append import allocate_bounds, append_kv, rope_cache
@@ -373,10 +372,3 @@ def test_other_streams_and_refused_arguments():
     with pytest.raises(ValueError, match="finite"):
         fp8_decode(g["q"], g["k"], g["v"], g["tables"], g["lengths"], resources=res,
                    scale=float("inf"))
-
-
-def test_split_counts_follow_the_batch_bucket():
-    for batch in (3, 4):
-        assert _native.block_splits(batch, 32, 8, 512, 256) == _native.block_splits(4, 32, 8, 512,
-                                                                                   256)
-    assert _native.block_splits(1, 8, 2, 3, 256) == 1
