@@ -419,7 +419,7 @@ struct DecodeArgs {
   float scale2;      // scale log2 e
 };
 
-// A wavefront's tile: kTile tokens, 8 KB of K and of V (at most 64 tokens).  S^T = K Q^T and
+// A wavefront's tile: kTile tokens, 8 KB of a bf16 K and V.  S^T = K Q^T and
 // O^T = V^T P^T with 16 x 16 x 32 MFMAs.  In both results a lane's column is query head
 // lane % 16, so the softmax state is one scalar a lane, and the layout of the scores (tokens
 // 16 u + 4 (lane / 16) + r in element r of result u) is the operand layout of P^T with its
@@ -431,7 +431,7 @@ struct DecodeArgs {
 template <int D, bool kE4m3>
 struct Decode {
   static constexpr int kBytes = kE4m3 ? 1 : 2;
-  static constexpr int kTile = D * kBytes >= 512 ? 16 : D * kBytes >= 256 ? 32 : 64;
+  static constexpr int kTile = kE4m3 ? 32 : 4096 / D;
   static constexpr int kSums = kTile / 16;               // results of S^T
   static constexpr int kGroups = kTile < 32 ? 1 : kTile / 32;
   static constexpr int kPer = kTile < 32 ? 4 : 8;        // tokens of a lane's P V operand
@@ -560,7 +560,7 @@ struct Tile {
 // The leading arguments are in registers when a wavefront starts, the others are loaded
 // while the length and the table are.
 template <int D, bool kE4m3>
-__global__ void __launch_bounds__(256, D == 128 && !kE4m3 ? 3 : 2)
+__global__ void __launch_bounds__(256, D == 256 || (D == 64 && !kE4m3) ? 2 : 3)
 block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restrict__ blocks,
                     const int32_t* __restrict__ table, int64_t tsb, int width, int kept, int hkv,
                     int num_pages, const char* __restrict__ k, const char* __restrict__ v,
@@ -583,27 +583,28 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
     x = id % gridDim.x, id /= gridDim.x;
     split = id % gridDim.y, b = id / gridDim.y;
   }
-  // With a head on the same XCD throughout, the rows that an XCD reads lie a token apart, in
-  // few of its L2's channels: the heads take turns.
-  x = uint32_t(x + kPair * (split + b)) % gridDim.x;
+  // The heads take turns on an XCD from sequence to sequence: where many workgroups follow
+  // one another, a head that stays on its XCD is slower (64 sequences of 16384 e4m3 tokens,
+  // Hkv 8, D 128, 8 splits: 441 and 386 us; 128 of 2048, Hkv 16, D 64: 137 and 111), where
+  // few do it is faster by 4 to 6% (one split: 423 and 451).
+  if (D == 64 || splits > 2) x = uint32_t(x + kPair * b) % gridDim.x;
   int g = x, head_tile = 0;
   if (int(gridDim.x) != hkv) g = x / p.tiles, head_tile = x % p.tiles;
   const int heads = min(p.group - 16 * head_tile, 16);
   const int head0 = g * p.group + 16 * head_tile;
 
-  // Tiles of the sequence, parts of its blocks or of the listed ones.  A split is whole
-  // rounds of the four wavefronts, the same for each of a sequence's splits.
+  // Tiles of the sequence, parts of its blocks or of the listed ones; the wavefronts of all
+  // its splits take them in turn, so that a short list's end is no split's alone.
   const int64_t len = min(int64_t(max(lengths[b], 0)), int64_t(width) * pd::kPageSize);
   const int count = blocks ? kParts * kept : int((len + kTile - 1) / kTile);
-  const int chunk = ((count + splits - 1) / splits + 3) & ~3;
-  const int s0 = split * chunk, s1 = min(s0 + chunk, count);
+  const int mine = split + splits * w, step_tiles = 4 * splits;
 
   floatx4_t o[T::kOut];
 #pragma unroll
   for (int i = 0; i < T::kOut; ++i) o[i] = floatx4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
 
-  if (s0 < s1) {
+  if (split < count) {
     u32x4_t q[T::kStepsQ];
     const uint16_t* qrow = q_rows + b * p.qsb + (head0 + min(col, heads - 1)) * p.qsh;
 #pragma unroll
@@ -689,12 +690,12 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
       next_v();
     };
 
-    // Tiles w, w + 4, ... of the split, 64 at a time, one a lane: its first slot / kTile and
-    // its live tokens (none: no such block or page).
-    for (int at = s0 + w; at < s1; at += 4 * 64) {
-      const int u = at + 4 * lane;
+    // The wavefront's tiles, 64 at a time, one a lane: its first slot / kTile and its live
+    // tokens (none: no such block or page).
+    for (int64_t at = mine; at < count; at += int64_t(64) * step_tiles) {
+      const int64_t u = at + int64_t(lane) * step_tiles;
       int first = 0, live = 0;
-      if (u < s1) {
+      if (u < count) {
         const int64_t j = blocks ? kParts * int64_t(blocks[(int64_t(b) * hkv + g) * kept + u / kParts]) +
                                        u % kParts
                                  : u;
@@ -868,8 +869,7 @@ many_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
 }
 
 int tile_tokens(int head_dim, int32_t cache_type) {
-  const int row = head_dim * (cache_type == PD_CACHE_E4M3 ? 1 : 2);
-  return row >= 512 ? 16 : row >= 256 ? 32 : 64;
+  return cache_type == PD_CACHE_E4M3 ? 32 : 4096 / head_dim;
 }
 
 int check_geometry(int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
@@ -963,14 +963,14 @@ extern "C" int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_
   int64_t rows = 1;
   while (rows < batch) rows *= 2;
   rows *= int64_t(num_kv_heads) * ((num_heads / num_kv_heads + 15) / 16);
-  // Listed blocks are as many for every row: one workgroup a CU, each with the most to do
-  // behind its start of some 3 us (17 rows of 37 blocks, Hq 32 / Hkv 4 / D 256, e4m3: 23.5 us;
-  // 26.9 with two, 30.2 with eight).  Whole caches differ in length: eight a CU, so that no
-  // long one is left to a few (64 of 1 to 32768 tokens, Hq 32 / Hkv 8 / D 128: 394 us; 604 with
-  // two; 8 of 1000 to 9000: 26.3 and 25.1).
+  // Listed blocks are about as many for every row: one workgroup a CU, each with the most to
+  // do behind its start of some 3 us (17 rows of 37 blocks, Hq 32 / Hkv 4 / D 256, e4m3: 22.6
+  // us; 28.5 with eight).  Whole caches differ in length: eight a CU, so that no long one is
+  // left to a few (64 of 1 to 32768 tokens, Hq 32 / Hkv 8 / D 128: 404 us; 604 with two; 8 of
+  // 1000 to 9000: 24.5 and 25.1).  Nor is a long list: 128 tiles a workgroup at most.
   const int64_t groups = int64_t(listed ? 1 : 8) * cus;
-  const int64_t want = (groups + rows - 1) / rows;
   const int64_t tiles = int64_t(entries) * (kBlock / tile_tokens(head_dim, cache_type));
+  const int64_t want = std::max((groups + rows - 1) / rows, tiles / 128);
   const int64_t most = std::min<int64_t>((tiles + 3) / 4, kMaxSplits);
   *splits = int32_t(std::max<int64_t>(1, std::min(want, most)));
   return PD_OK;
