@@ -43,12 +43,11 @@ __device__ __forceinline__ int block_count(const int32_t* lengths, int b, int wi
 // block: two implementations pick the same ones unless their scores agree to 15
 // digits without being equal.
 struct SelectArgs {
+  const int32_t *lengths, *table;
   const uint16_t *q, *bounds;
-  const int32_t *table, *lengths;
   uint64_t* keys;  // [batch][hkv][width * 4]
-  int32_t* blocks;
-  int64_t qsb, qsh, tsb, num_pages;
-  int width, hkv, group, kept, first, last;
+  int64_t qsb, qsh, tsb;
+  int width, hkv, num_pages, group, kept, first, last;
 };
 
 // Larger for a larger score; a NaN counts as +infinity, -0 as +0.
@@ -95,6 +94,7 @@ struct Bounds {
   u32x4_t lo, hi;
   bool known;
   __device__ __forceinline__ void load(const SelectArgs& p, int b, int g, int j, int part) {
+    j = min(j, p.width * kPerPage - 1);  // past the last candidate: any entry, not used
     const int64_t page = p.table[b * p.tsb + j / kPerPage];
     known = page >= 0 && page < p.num_pages;
     const uint16_t* at =
@@ -144,22 +144,22 @@ __device__ __forceinline__ double best_of(const Query<D, kHeads>& q, const doubl
   return x;
 }
 
-// Scores of blocks j0 + w kPer + lane / kLanes, every `step` blocks, below `end`, to
-// store(j, key).  kHeads >= group: the query stays in registers; else it is taken again for
-// every run, kHeads heads at a time.
-template <int D, int kHeads, bool kWhole, typename Store>
+// Scores of blocks j0 + lane / kLanes, every `step` blocks, below end_of(), which waits for the
+// length, to store(j, key).  kWhole (kHeads >= group): the query stays in registers; else it
+// is taken again for every run, kHeads heads at a time.
+template <int D, int kHeads, bool kWhole, typename End, typename Store>
 __device__ __forceinline__ void score_blocks(const SelectArgs& p, int b, int g, int j0, int step,
-                                             int end, int lane, Store store) {
+                                             int lane, End end_of, Store store) {
   using S = Scores<D>;
   const int part = lane % S::kLanes, mine = lane / S::kLanes;
-  if (j0 >= end) return;
   Bounds<D> next;
-  next.load(p, b, g, min(j0 + mine, end - 1), part);
+  next.load(p, b, g, j0 + mine, part);
   Query<D, kHeads> q;
   if constexpr (kWhole) q.load(p, b, g, 0, part);
+  const int end = end_of();
   for (int j = j0; j < end; j += step) {
     const Bounds<D> here = next;
-    if (j + step < end) next.load(p, b, g, min(j + step + mine, end - 1), part);
+    if (j + step < end) next.load(p, b, g, j + step + mine, part);
     double mid[8], radius[8];
     float lo[8], hi[8];
     unpack8(here.lo, lo);
@@ -185,16 +185,23 @@ __device__ __forceinline__ void score_blocks(const SelectArgs& p, int b, int g, 
 
 // The scores of one (sequence, kv head), cut over the workgroups of grid.x.
 template <int D, int kHeads, bool kWhole>
-__global__ void __launch_bounds__(256) score_kernel(const SelectArgs p) {
+__global__ void __launch_bounds__(256)
+score_kernel(const int32_t* lengths, const int32_t* table, const uint16_t* q,
+             const uint16_t* bounds, uint64_t* keys_of, int64_t tsb, int width, int hkv,
+             int num_pages, int kept, int first, int last, int group, int64_t qsb, int64_t qsh) {
+  const SelectArgs p{lengths, table, q,     bounds, keys_of, qsb,   qsh, tsb,
+                     width,   hkv,   num_pages, group, kept,    first, last};
   constexpr int kPer = Scores<D>::kPer;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int g = blockIdx.y, b = blockIdx.z;
-  const int n = block_count(p.lengths, b, p.width);
-  if (n <= p.kept) return;
   uint64_t* keys = p.keys + (int64_t(b) * p.hkv + g) * p.width * kPerPage;
-  score_blocks<D, kHeads, kWhole>(p, b, g, p.first + (blockIdx.x * 4 + w) * kPer,
-                                  gridDim.x * 4 * kPer, n - p.last, lane,
-                                  [&](int j, uint64_t key) { keys[j] = key; });
+  score_blocks<D, kHeads, kWhole>(
+      p, b, g, p.first + (blockIdx.x * 4 + w) * kPer, gridDim.x * 4 * kPer, lane,
+      [&] {
+        const int n = block_count(p.lengths, b, p.width);
+        return n > p.kept ? n - p.last : 0;
+      },
+      [&](int j, uint64_t key) { keys[j] = key; });
 }
 
 template <int M>
@@ -219,16 +226,14 @@ struct Picker {
   uint64_t edge;
 };
 
-// kCache > 0: a thread's keys, at most that many, stay in its registers.
-template <int kWaves, int kCache>
+// kAll: `cached` holds all of the thread's keys, begin + its number + i threads of them.
+template <int kWaves, bool kAll>
 __device__ __forceinline__ void pick_blocks(Picker<kWaves>& t, const uint64_t* __restrict__ keys,
-                                            int n, int begin, int end, uint32_t need,
-                                            int32_t* out) {
+                                            const uint64_t (&cached)[kCached], int n, int begin,
+                                            int end, uint32_t need, int32_t* out) {
+  constexpr int kCache = kAll ? kCached : 0;
   constexpr int kThreads = 64 * kWaves;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  uint64_t cached[kCache + 1];
-#pragma unroll
-  for (int i = 0; i < kCache; ++i) cached[i] = keys[min(begin + tid + i * kThreads, end - 1)];
   const auto each = [&](auto use) {  // use(j, key) of the thread's candidates
     if constexpr (kCache > 0) {
 #pragma unroll
@@ -271,7 +276,7 @@ __device__ __forceinline__ void pick_blocks(Picker<kWaves>& t, const uint64_t* _
       each([&](int j, uint64_t key) {
         if (key >> shift == edge) {
           const uint32_t at = atomicAdd(&t.close, 1u);
-          t.close_keys[at] = key, t.close_blocks[at] = j;
+          if (at < 64) t.close_keys[at] = key, t.close_blocks[at] = j;
         }
       });
       __syncthreads();
@@ -351,7 +356,7 @@ __device__ __forceinline__ void pick_blocks(Picker<kWaves>& t, const uint64_t* _
     // Ties ahead of this block that are in: the first `need` of them.
     const uint32_t tied = ties + (ahead >> 16) + __popcll(__ballot(tie) & below);
     const uint32_t at = written + (ahead & 0xffff) + __popcll(__ballot(in) & below) + min(tied, need);
-    if (in || (tie && tied < need)) out[at] = j;
+    if ((in || (tie && tied < need)) && at < begin + taken) out[at] = j;
     written += all & 0xffff;
     ties += all >> 16;
   };
@@ -393,19 +398,27 @@ __device__ __forceinline__ void list_all(int32_t* out, int kept, int n) {
 // 16, whose barriers cost more than their keys.
 constexpr int kPickWaves = 4;
 
-__global__ void __launch_bounds__(64 * kPickWaves) pick_kernel(const SelectArgs p) {
+__global__ void __launch_bounds__(64 * kPickWaves)
+pick_kernel(const int32_t* __restrict__ lengths, const uint64_t* __restrict__ all_keys,
+            int32_t* __restrict__ blocks, int width, int hkv, int kept, int first, int last) {
   __shared__ Picker<kPickWaves> picker;
   const int g = blockIdx.x, b = blockIdx.y;
-  const int n = block_count(p.lengths, b, p.width);
-  int32_t* out = p.blocks + (int64_t(b) * p.hkv + g) * p.kept;
-  if (n <= p.kept) return list_all(out, p.kept, n);
-  const uint64_t* keys = p.keys + (int64_t(b) * p.hkv + g) * p.width * kPerPage;
-  const int begin = p.first, end = n - p.last;
-  const uint32_t need = uint32_t(p.kept - p.first - p.last);
-  if (end - begin <= kCached * 64 * kPickWaves)
-    pick_blocks<kPickWaves, kCached>(picker, keys, n, begin, end, need, out);
+  const uint64_t* keys = all_keys + (int64_t(b) * hkv + g) * width * kPerPage;
+  // A thread's first keys are on their way while the length is.
+  uint64_t cached[kCached];
+#pragma unroll
+  for (int i = 0; i < kCached; ++i)
+    cached[i] = keys[min(int64_t(first) + int(threadIdx.x) + i * 64 * kPickWaves,
+                         int64_t(width) * kPerPage - 1)];
+  const int n = block_count(lengths, b, width);
+  int32_t* out = blocks + (int64_t(b) * hkv + g) * kept;
+  if (n <= kept) return list_all(out, kept, n);
+  const int end = n - last;
+  const uint32_t need = uint32_t(kept - first - last);
+  if (end - first <= kCached * 64 * kPickWaves)
+    pick_blocks<kPickWaves, true>(picker, keys, cached, n, first, end, need, out);
   else
-    pick_blocks<kPickWaves, 0>(picker, keys, n, begin, end, need, out);
+    pick_blocks<kPickWaves, false>(picker, keys, cached, n, first, end, need, out);
 }
 
 // ------------------------------------------------------------------ attention
@@ -595,9 +608,25 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
 
   // Tiles of the sequence, parts of its blocks or of the listed ones; the wavefronts of all
   // its splits take them in turn, so that a short list's end is no split's alone.
-  const int64_t len = min(int64_t(max(lengths[b], 0)), int64_t(width) * pd::kPageSize);
-  const int count = blocks ? kParts * kept : int((len + kTile - 1) / kTile);
   const int mine = split + splits * w, step_tiles = 4 * splits;
+  // Tile u, one a lane (below 0: no block of the table), and its page; the first of them are
+  // looked up while the length is on its way.
+  struct Place {
+    int tile, page;
+  };
+  const auto look = [&](int u) {
+    Place at;
+    at.tile = u;
+    if (blocks) {
+      const int j = blocks[(int64_t(b) * hkv + g) * kept + min(u / kParts, kept - 1)];
+      at.tile = uint32_t(j) < uint32_t(width * kPerPage) ? kParts * j + u % kParts : -1;
+    }
+    at.page = table[b * tsb + min(max(at.tile, 0) / kTiles, width - 1)];
+    return at;
+  };
+  Place here = look(mine + lane * step_tiles);
+  const int len = min(max(lengths[b], 0), width * pd::kPageSize);  // width below 2^22
+  const int count = blocks ? kParts * kept : (len + kTile - 1) / kTile;
 
   floatx4_t o[T::kOut];
 #pragma unroll
@@ -690,24 +719,14 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
       next_v();
     };
 
-    // The wavefront's tiles, 64 at a time, one a lane: its first slot / kTile and its live
-    // tokens (none: no such block or page).
-    for (int64_t at = mine; at < count; at += int64_t(64) * step_tiles) {
-      const int64_t u = at + int64_t(lane) * step_tiles;
-      int first = 0, live = 0;
-      if (u < count) {
-        const int64_t j = blocks ? kParts * int64_t(blocks[(int64_t(b) * hkv + g) * kept + u / kParts]) +
-                                       u % kParts
-                                 : u;
-        const int64_t left = len - j * kTile;
-        if (j >= 0 && left > 0) {
-          const int page = table[b * tsb + uint32_t(j) / kTiles];
-          if (page >= 0 && page < num_pages) {
-            first = page * kTiles + int(uint32_t(j) % kTiles);
-            live = left < kTile ? int(left) : kTile;
-          }
-        }
-      }
+    for (int at = mine; at < count; at += 64 * step_tiles) {
+      if (at != mine) here = look(at + lane * step_tiles);
+      // Live tokens of the lane's tile (none: no such block or page).
+      const bool known = at + lane * step_tiles < count && here.tile >= 0 && here.page >= 0 &&
+                         here.page < num_pages;
+      const int left = len - here.tile * kTile;
+      const int live = known ? min(max(left, 0), kTile) : 0;
+      const int first = live ? here.page * kTiles + here.tile % kTiles : 0;
       const uint64_t any = __ballot(live > 0);
       if (!any) continue;
       const int last = 63 - __builtin_clzll(any);
@@ -715,13 +734,13 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
         return int64_t(uint32_t(__builtin_amdgcn_readlane(first, i))) * kTile * token +
                int64_t(g) * D * T::kBytes;
       };
-      int64_t here = offset(0);
-      t.load_k(k + here, token, lane);
-      t.load_v(v + here, token, lane);
+      int64_t from = offset(0);
+      t.load_k(k + from, token, lane);
+      t.load_v(v + from, token, lane);
       for (int i = 0; i < last; ++i) {
-        here = offset(i + 1);
-        step(__builtin_amdgcn_readlane(live, i), [&] { t.load_k(k + here, token, lane); },
-             [&] { t.load_v(v + here, token, lane); });
+        from = offset(i + 1);
+        step(__builtin_amdgcn_readlane(live, i), [&] { t.load_k(k + from, token, lane); },
+             [&] { t.load_v(v + from, token, lane); });
       }
       step(__builtin_amdgcn_readlane(live, last), [] {}, [] {});
     }
@@ -909,11 +928,7 @@ extern "C" int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_str
     return pd::fail(PD_EINVAL, "tensors must be present, query rows and bounds 16-byte aligned");
   if (batch > 65535 || num_kv_heads > 65535)
     return pd::fail(PD_EINVAL, "grid dimension exceeds device limits");
-  SelectArgs p;
-  p.q = u16(q), p.bounds = u16(bounds), p.table = table, p.lengths = lengths, p.keys = keys;
-  p.blocks = blocks, p.qsb = q_stride_b, p.qsh = q_stride_h, p.tsb = table_stride_b;
-  p.num_pages = num_pages, p.width = table_width, p.hkv = num_kv_heads;
-  p.group = num_heads / num_kv_heads, p.kept = kept, p.first = first, p.last = last;
+  const int group = num_heads / num_kv_heads;
   const int64_t wide = int64_t(table_width) * kPerPage;
   if (wide > kept) {
     const auto go = [&](auto dim, auto heads, auto whole) {
@@ -926,14 +941,16 @@ extern "C" int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_str
       const int64_t most = std::max<int64_t>(1, 2048 / (int64_t(batch) * num_kv_heads));
       hipLaunchKernelGGL((score_kernel<dim.value, heads.value, whole.value>),
                          dim3(unsigned(std::min(groups, most)), num_kv_heads, batch), dim3(256), 0,
-                         as_stream(stream), p);
+                         as_stream(stream), lengths, table, u16(q), u16(bounds), keys,
+                         table_stride_b, table_width, num_kv_heads, int(num_pages), kept, first,
+                         last, group, q_stride_b, q_stride_h);
     };
     const auto with = [&](auto dim) {
-      if (p.group == 1)
+      if (group == 1)
         go(dim, std::integral_constant<int, 1>{}, std::true_type{});
-      else if (p.group == 2)
+      else if (group == 2)
         go(dim, std::integral_constant<int, 2>{}, std::true_type{});
-      else if (p.group <= 4)
+      else if (group <= 4)
         go(dim, std::integral_constant<int, 4>{}, std::true_type{});
       else
         go(dim, std::integral_constant<int, 4>{}, std::false_type{});
@@ -947,7 +964,8 @@ extern "C" int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_str
     if (const int bad = launch_status("pd_select_blocks")) return bad;
   }
   hipLaunchKernelGGL(pick_kernel, dim3(num_kv_heads, batch), dim3(64 * kPickWaves), 0,
-                     as_stream(stream), p);
+                     as_stream(stream), lengths, keys, blocks, table_width, num_kv_heads, kept,
+                     first, last);
   return launch_status("pd_select_blocks");
 }
 
@@ -1007,12 +1025,21 @@ extern "C" int pd_block_decode(const void* q, int64_t q_stride_b, int64_t q_stri
     return pd::fail(PD_EINVAL, "grid dimension exceeds device limits");
   const dim3 grid = {unsigned(columns), unsigned(splits), unsigned(batch)};
   const unsigned lds = unsigned(128 + 4 * (p.group < 16 ? p.group : 16) * head_dim) * 4;
+  bool fits = true;
   pd::for_cache(head_dim, cache_type, [&](auto dim, auto e4m3) {
-    hipLaunchKernelGGL((block_decode_kernel<dim.value, e4m3.value>), grid, dim3(256), lds,
+    const auto kernel = block_decode_kernel<dim.value, e4m3.value>;
+    if (lds > 64 * 1024 &&
+        hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)) != hipSuccess) {
+      fits = false;
+      return;
+    }
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds,
                        as_stream(stream), lengths, blocks, table, table_stride_b, table_width,
                        kept, num_kv_heads, int(num_pages), static_cast<const char*>(k),
                        static_cast<const char*>(v), u16(q), p);
   });
+  if (!fits) return pd::fail(PD_ELAUNCH, "pd_block_decode: LDS size");
   if (const int bad = launch_status("pd_block_decode")) return bad;
   if (splits == 1) return PD_OK;
   if (splits <= kFewSplits) {

@@ -157,6 +157,8 @@ def select_blocks(q, bounds, tables, lengths, *, resources, first=1, last=1):
     spec, blocks = resources.spec, resources.blocks
     if not resources.kept:
         raise ValueError("these resources hold no list of blocks: allocate them with kept=")
+    if first < 0 or last < 1 or first + last > resources.kept:
+        raise ValueError("kept blocks must hold the first ones and at least one last")
     hkv, dim, shape = spec.num_kv_heads, spec.head_dim, bounds.shape
     if (shape[1:] != (_PER_PAGE, hkv, 2, dim) or bounds.dtype != torch.bfloat16
             or not bounds.is_contiguous() or bounds.get_device() != device or shape[0] == 0):
