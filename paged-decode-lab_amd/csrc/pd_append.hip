@@ -401,7 +401,7 @@ extern "C" int pd_append_kv(const void* q, int64_t q_stride, const void* k, int6
   const int64_t strides[4] = {q_stride, q_out_stride, k_stride, v_stride};
   const int64_t least[4] = {0, int64_t(num_heads) * head_dim, 0, 0};
   for (int i = 0; i < 4; ++i)
-    if ((i > 1 || num_heads) && (strides[i] % 8 || strides[i] < least[i]))
+    if (rows > 1 && (i > 1 || num_heads) && (strides[i] % 8 || strides[i] < least[i]))
       return pd::fail(PD_EINVAL, "row strides must be non-negative multiples of 8, of q_out at "
                                  "least a row");
   if (!all_aligned16(q, k, v, rope, q_out, k_cache, v_cache, bounds))

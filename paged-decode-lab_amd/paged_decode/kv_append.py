@@ -93,9 +93,9 @@ def append_kv(q, k, v, positions, rope, k_cache, v_cache, slot_mapping, *, inter
     """Rotated queries [N, Hq, D]; keys (rotated) and values written to their slots.
 
     q [N, Hq, D] (or None: returns None), k and v [N, Hkv, D] bf16, heads contiguous; rows may
-    be slices of a fused projection.  ``rope`` float32 [M, half, 2] (``rope_cache``) and ``positions`` int64
-    [N]: element pairs (j, j + half), or (2j, 2j + 1) with ``interleaved``, of the leading
-    2 half elements are rotated, half a multiple of 8; rope None rotates nothing.
+    be slices of a fused projection.  ``rope`` float32 [M, half, 2] (``rope_cache``) and
+    ``positions`` int64 [N]: element pairs (j, j + half), or (2j, 2j + 1) with ``interleaved``,
+    of the leading 2 half elements are rotated, half a multiple of 8; rope None rotates nothing.
     Caches [blocks, block_size, Hkv, D] bf16 or float8_e4m3fn, which holds x / scale, clamped
     to +-448; ``slot_mapping`` int32 [N], a negative slot (or one past the cache) writes
     nothing, slots of one call must differ.  A position outside the table writes nothing and
@@ -105,8 +105,14 @@ def append_kv(q, k, v, positions, rope, k_cache, v_cache, slot_mapping, *, inter
     if len(shape) != 3 or device < 0:
         _refuse("key must be [N, kv_heads, head_dim] on a CUDA device")
     n, hkv, dim = shape
-    k_stride = _row_stride(k, n, hkv, dim, device, "key")
-    v_stride = _row_stride(v, n, hkv, dim, device, "value")
+    k_stride, v_stride = k.stride(), v.stride()
+    if v.shape != shape:
+        _refuse("value must have the key's shape")
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        _refuse("BF16 query/key/value required")
+    if (k_stride[2] != 1 or v_stride[2] != 1
+            or (hkv != 1 and (k_stride[1] != dim or v_stride[1] != dim))):
+        _refuse("key and value heads must be contiguous")
     cache, kind = k_cache.shape, k_cache.dtype
     cache_type = _native.CACHE_TYPES.get(kind)
     if cache_type is None or v_cache.dtype != kind:
@@ -115,7 +121,7 @@ def append_kv(q, k, v, positions, rope, k_cache, v_cache, slot_mapping, *, inter
             or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
         _refuse("caches must be contiguous [blocks, block_size, kv_heads, head_dim] with the "
                 "key's heads")
-    if k_cache.get_device() != device or v_cache.get_device() != device:
+    if not k_cache.get_device() == v_cache.get_device() == v.get_device() == device:
         _refuse("all tensors must be on one CUDA device")
     _check_index(slot_mapping, n, torch.int32, device, "slot_mapping")
     if k_scale is not None or v_scale is not None:
@@ -143,11 +149,11 @@ def append_kv(q, k, v, positions, rope, k_cache, v_cache, slot_mapping, *, inter
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad
                                     or (q is not None and q.requires_grad)):
         _refuse("append_kv has no gradient: call it under torch.no_grad()")
-    _native.launch(device, _native.lib().pd_append_kv, _pointer(q), q_stride, k.data_ptr(), k_stride,
-                   v.data_ptr(), v_stride, *table, interleaved, _pointer(out), out_stride,
-                   k_cache.data_ptr(), v_cache.data_ptr(), cache_type, cache[0] * cache[1],
-                   slot_mapping.data_ptr(), _pointer(k_scale), _pointer(v_scale), _pointer(bounds),
-                   n, heads, hkv, dim)
+    _native.launch(device, _native.lib().pd_append_kv, _pointer(q), q_stride, k.data_ptr(),
+                   k_stride[0], v.data_ptr(), v_stride[0], *table, interleaved, _pointer(out),
+                   out_stride, k_cache.data_ptr(), v_cache.data_ptr(), cache_type,
+                   cache[0] * cache[1], slot_mapping.data_ptr(), _pointer(k_scale),
+                   _pointer(v_scale), _pointer(bounds), n, heads, hkv, dim)
     return out
 
 

@@ -226,3 +226,68 @@ def test_captured_steps_replay_with_new_rows(kind):
         assert torch.equal(bits(x["k_cache"]), bits(y["k_cache"]))
         assert torch.equal(bits(x["v_cache"]), bits(y["v_cache"]))
         assert torch.equal(bits(bounds), bits(eager_bounds))
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("half,interleaved", [(0, False), (32, False), (64, True)])
+@pytest.mark.parametrize("n", [200, 513, 700])
+def test_bounds_of_rows_in_any_order(n, half, interleaved, kind):
+    """Whole and part blocks with their rows permuted, some rows not written: padded slots and
+    positions outside the table, whose keys stay the cache's own."""
+    x = make(n, 8, 2, 128, half, kind, seed=n + half, start=70)
+    order = torch.from_numpy(np.random.default_rng(n).permutation(n)).cuda()
+    for name in ("q", "k", "v", "positions", "slots"):
+        x[name] = x[name][order]
+    x["slots"][5] = -1
+    if half:
+        x["positions"][[17, 30]] = torch.tensor([-1, 600], device="cuda")
+    bounds = torch.full_like(allocate_bounds(x["k_cache"]), 77.0)
+    call(x, bounds=bounds, interleaved=interleaved)
+    torch.cuda.synchronize()
+    keys = x["k_cache"].cpu().view(-1, 64, 2, 128)
+    want = torch.full((len(keys), 2, 2, 128), 77.0, dtype=torch.bfloat16)
+    for slot in x["slots"].tolist():
+        if slot >= 0 and slot % 64 == 63:
+            want[slot // 64] = O.block_bounds(keys[slot // 64])
+    assert torch.equal(bounds.cpu().view(want.shape).float(), want.float())
+
+
+def test_one_row_of_any_stride():
+    x = make(1, 8, 2, 128, 64, torch.bfloat16, seed=31)
+    q, k_bits, v_bits, _ = expected(x)
+    for name in ("q", "k", "v"):
+        x[name] = torch.as_strided(x[name].contiguous(), x[name].shape, (3, 128, 1))
+    out = call(x)
+    assert torch.equal(bits(out), bits(q))
+    assert torch.equal(bits(x["k_cache"]), k_bits) and torch.equal(bits(x["v_cache"]), v_bits)
+
+
+def test_refused_tensors():
+    x = make(4, 8, 2, 128, 64, E4M3, seed=32)
+    bounds = allocate_bounds(x["k_cache"])
+    cases = [(dict(k=x["k"].float()), "BF16"), (dict(v=x["v"][:3]), "shape"),
+             (dict(q=x["q"].transpose(1, 2)), "head_dim|heads"), (dict(q=x["q"].float()), "BF16"),
+             (dict(k=x["k"].transpose(1, 2).contiguous().transpose(1, 2)), "contiguous"),
+             (dict(slots=x["slots"].long()), "int32"), (dict(slots=x["slots"][:3]), "one entry"),
+             (dict(positions=x["positions"].int()), "int64"), (dict(slots=x["slots"].cpu()), "device"),
+             (dict(rope=x["rope"].double()), "rope"), (dict(rope=x["rope"].transpose(0, 1)), "rope"),
+             (dict(k_cache=x["k_cache"].float()), "float8"),
+             (dict(k_cache=x["k_cache"].view(torch.uint8)), "float8"),
+             (dict(k_cache=x["k_cache"][:, :, :1]), "heads"), (dict(v_cache=x["v_cache"][:1]), "heads"),
+             (dict(k_scale=torch.ones(3, device="cuda")), "scales"),
+             (dict(v_scale=torch.ones(2)), "scales"),
+             (dict(k_cache=x["k_cache"].bfloat16(), v_cache=x["v_cache"].bfloat16()), "scales")]
+    for change, message in cases:
+        with pytest.raises(ValueError, match=message):
+            call(dict(x, **change))
+    for bad in (bounds.float(), bounds[:2], bounds.transpose(2, 3)):
+        with pytest.raises(ValueError, match="bounds"):
+            call(x, bounds=bad)
+    with pytest.raises(ValueError, match="rows"):
+        call(x, out=torch.empty((3, 8, 128), dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError, match="needs a query"):
+        call(dict(x, q=None), out=x["q"])
+    with pytest.raises(ValueError, match="no gradient"):
+        call(dict(x, k=x["k"].clone().requires_grad_()))
+    with pytest.raises(ValueError, match="multiple of 8"):
+        call(dict(x, rope=x["rope"][:, :12].contiguous()))

@@ -71,7 +71,7 @@ def check(got, x, blocks=None, **more):
 LENGTHS = [[1], [0, 1, 31, 32, 33, 63, 64, 65, 127, 255, 256, 257], [700, 0, 2064, 1500],
            [5000], [64 * 97]]
 HEADS = [(16, 4, 256), (32, 8, 128), (16, 16, 64), (8, 2, 128), (4, 4, 256), (17, 1, 64),
-         (40, 2, 128), (16, 1, 256)]
+         (40, 2, 128), (16, 1, 256), (6, 3, 64)]
 
 
 @pytest.mark.parametrize("hq,hkv,d", HEADS)
@@ -372,3 +372,81 @@ def test_other_streams_and_refused_arguments():
     with pytest.raises(ValueError, match="finite"):
         fp8_decode(g["q"], g["k"], g["v"], g["tables"], g["lengths"], resources=res,
                    scale=float("inf"))
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 8, 9, 16, 17, 33, 64, 100, 128])
+def test_every_split_count_gives_the_same_attention(splits, kind):
+    """Splits set by hand: more than the plan's and fewer, so that a wavefront's tiles are none,
+    one, or more than it looks up at once (64)."""
+    lengths = [0, 1, 33, 700, 9300]
+    x = make(lengths, 8, 2, 128, kind, seed=71)
+    g = dev(x)
+    kept = 146
+    blocks = torch.arange(kept, dtype=torch.int32).expand(5, 2, kept).contiguous()
+    res = allocate_block_resources(spec_of(x), "cuda", kept=kept)
+    res._splits[5, kind] = splits
+    res.partials = torch.full((5 * 8 * splits * 128,), float("nan"), device="cuda")
+    res.sums = torch.full((5 * 8 * splits * 2,), float("nan"), device="cuda")
+    check(attend(x, g, res, blocks.cuda()), x, blocks)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.05, 0.3])
+def test_scales_of_the_scores(scale):
+    x = make([500, 70], 8, 2, 128, E4M3, seed=72)
+    g = dev(x)
+    res = allocate_block_resources(spec_of(x), "cuda")
+    out = fp8_decode(g["q"], g["k"], g["v"], g["tables"], g["lengths"], resources=res, scale=scale,
+                     k_scale=g["k_scale"], v_scale=g["v_scale"])
+    check(out, x, scale=scale)
+
+
+def test_select_from_more_blocks_than_a_workgroup_holds():
+    pages = 590
+    tables = torch.from_numpy(np.random.default_rng(2).permutation(pages).astype(np.int32)[None])
+    gen = torch.Generator().manual_seed(73)
+    lengths = torch.tensor([150_001], dtype=torch.int32)
+    res = allocate_block_resources(DecodeSpec(1, 4, 2, 64, pages * 256), "cuda", kept=300)
+    for integers in (False, True):
+        shape = (pages, 4, 2, 1, 64)
+        low = torch.randint(-2, 2, shape, generator=gen).float() if integers \
+            else torch.randn(shape, generator=gen)
+        bounds = torch.cat([low, low + torch.rand(shape, generator=gen).round()], 3).bfloat16()
+        q = torch.randn((1, 4, 64), generator=gen)
+        q = (q.round() if integers else q).bfloat16()
+        got = select_blocks(q.cuda(), bounds.cuda(), tables.cuda(), lengths.cuda(), resources=res)
+        assert torch.equal(got.cpu(), O.select(q, bounds, tables, lengths, 300))
+
+
+def test_two_graphs_share_their_resources():
+    """Captured with the same workspaces, replayed in turn on one stream."""
+    x = make([3000, 1200], 8, 2, 128, torch.bfloat16, seed=74)
+    g = dev(x)
+    bounds = bounds_of(x, 74).cuda()
+    res = allocate_block_resources(spec_of(x), "cuda", kept=8)
+    graphs = []
+    for i in range(2):
+        q = g["q"].clone() if i else g["q"].neg()
+        args = dict(g, q=q)
+
+        def step():
+            blocks = select_blocks(q, bounds, g["tables"], g["lengths"], resources=res)
+            return blocks.clone(), attend(x, args, res, blocks).clone()
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        want = [t.clone() for t in want]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graphs.append((graph, got, want, q))      # the graph reads q
+    assert not torch.equal(graphs[0][2][0], graphs[1][2][0])
+    for i in (0, 1, 1, 0, 0, 1):
+        graph, got, want, _ = graphs[i]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
