@@ -423,12 +423,29 @@ pick_kernel(const int32_t* __restrict__ lengths, const uint64_t* __restrict__ al
 
 // ------------------------------------------------------------------ attention
 
+// Splits that a sequence of `len` tokens uses: as many as leave every wavefront a tile of it
+// (of the list, where that has fewer), or two.  The others end at once.  A table's width is a
+// capacity: 64 sequences of 500 to 1500 tokens with room for 131072 take 45 us, 34 with room
+// for 1500, and 81 in as many splits as there are.
+struct SplitRule {
+  int width, listed, tile, two, splits;  // listed: tiles of a list, 0: every block
+  __device__ __forceinline__ int length(const int32_t* lengths, int b) const {
+    return min(max(lengths[b], 0), width * pd::kPageSize);  // width below 2^22
+  }
+  __device__ __forceinline__ int used(int len) const {
+    const int filled = (len + tile - 1) >> __builtin_ctz(tile);
+    const int count = listed ? min(listed, filled) : filled;
+    return max(1, min(splits, (count + (4 << two) - 1) >> (2 + two)));
+  }
+};
+
 struct DecodeArgs {
   const float *k_scale, *v_scale;
   float *part_o, *part_ml;  // [batch][heads][splits][D], [batch][heads][splits][2]
   uint16_t* out;
   int64_t qsb, qsh;
   int group, tiles;  // tiles: of 16 query heads a kv head
+  int two;           // SplitRule's
   float scale2;      // scale log2 e
 };
 
@@ -608,7 +625,6 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
 
   // Tiles of the sequence, parts of its blocks or of the listed ones; the wavefronts of all
   // its splits take them in turn, so that a short list's end is no split's alone.
-  const int mine = split + splits * w, step_tiles = 4 * splits;
   // Tile u, one a lane (below 0: no block of the table), and its page; the first of them are
   // looked up while the length is on its way.
   struct Place {
@@ -624,9 +640,13 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
     at.page = table[b * tsb + min(max(at.tile, 0) / kTiles, width - 1)];
     return at;
   };
-  Place here = look(mine + lane * step_tiles);
-  const int len = min(max(lengths[b], 0), width * pd::kPageSize);  // width below 2^22
+  Place here = look(split + splits * (w + 4 * lane));
+  const SplitRule rule{width, blocks ? kParts * kept : 0, kTile, p.two, splits};
+  const int len = rule.length(lengths, b), used = rule.used(len);
+  if (split >= used) return;
+  if (used != splits) here = look(split + used * (w + 4 * lane));
   const int count = blocks ? kParts * kept : (len + kTile - 1) / kTile;
+  const int mine = split + used * w, step_tiles = 4 * used;
 
   floatx4_t o[T::kOut];
 #pragma unroll
@@ -779,7 +799,7 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += cell[(j * T::kOut + e) * 16 * heads];
     }
-    if (splits == 1) {
+    if (used == 1) {
       sum *= (kE4m3 && p.v_scale ? p.v_scale[g] : 1.f) / (hl == 0.f ? 1.f : hl);
       *reinterpret_cast<u32x2_t*>(p.out + (first + h) * D + d) =
           u32x2_t{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
@@ -791,8 +811,8 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
   }
 }
 
-// out = sum of the splits' o 2^(m - M) over that of their l, times v_scale.  An empty
-// split has l = 0, and its o is not there.
+// out = sum of the used splits' o 2^(m - M) over that of their l, times v_scale.  A split
+// without tokens has l = 0, and its o is not there; one used split has written the output.
 constexpr int kMaxSplits = PD_BLOCK_SPLITS;
 constexpr int kFewSplits = 8;
 
@@ -801,18 +821,22 @@ constexpr int kFewSplits = 8;
 template <int kMost>
 __global__ void __launch_bounds__(256)
 few_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                 uint16_t* __restrict__ out, int splits, int dim, int64_t total,
-                 const float* __restrict__ v_scale, int group, int heads) {
+                 uint16_t* __restrict__ out, const int32_t* __restrict__ lengths,
+                 const SplitRule rule, int dim, int64_t total, const float* __restrict__ v_scale,
+                 int group, int heads) {
+  const int splits = rule.splits;
   const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
   if (at >= total) return;
   const int64_t bh = at / dim;
   const int col = int(at - bh * dim);
+  const int used = rule.used(rule.length(lengths, int(bh / heads)));
+  if (used == 1) return;
   floatx2_t ml[kMost];
   floatx4_t o[kMost];
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kMost; ++i) {
-    const int64_t from = bh * splits + min(i, splits - 1);
+    const int64_t from = bh * splits + min(i, used - 1);
     ml[i] = *reinterpret_cast<const floatx2_t*>(part_ml + 2 * from);
     o[i] = *reinterpret_cast<const floatx4_t*>(part_o + from * dim + col);
     top = fmaxf(top, ml[i][0]);
@@ -822,7 +846,7 @@ few_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ par
   float l = 0.f;
 #pragma unroll
   for (int i = 0; i < kMost; ++i) {
-    const bool real = i < splits && ml[i][1] != 0.f;
+    const bool real = i < used && ml[i][1] != 0.f;
     const float f = exp2_fast(ml[i][0] - base);
     l += real ? f * ml[i][1] : 0.f;
 #pragma unroll
@@ -839,8 +863,10 @@ constexpr int kMergeCols = 64;
 template <int kMost>
 __global__ void __launch_bounds__(256)
 many_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                  uint16_t* __restrict__ out, int splits, int dim,
-                  const float* __restrict__ v_scale, int group, int heads) {
+                  uint16_t* __restrict__ out, const int32_t* __restrict__ lengths,
+                  const SplitRule rule, int dim, const float* __restrict__ v_scale, int group,
+                  int heads) {
+  const int splits = rule.splits;
   constexpr int kLanes = kMergeCols / 4, kRows = 256 / kLanes;
   __shared__ float weight[kMaxSplits];
   __shared__ float waves[4][2];
@@ -849,14 +875,16 @@ many_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
   const int64_t bh = blockIdx.x;
   const int col = blockIdx.y * kMergeCols + 4 * (tid % kLanes), row = tid / kLanes;
   const float* mine = part_o + bh * splits * dim + col;
+  const int used = rule.used(rule.length(lengths, int(bh / heads)));
+  if (used == 1) return;
   // The rows are on their way while the weights are made.
   floatx4_t o[kMost];
 #pragma unroll
   for (int i = 0; i < kMost; ++i)
     o[i] = *reinterpret_cast<const floatx4_t*>(mine +
-                                               int64_t(min(row + i * kRows, splits - 1)) * dim);
+                                               int64_t(min(row + i * kRows, used - 1)) * dim);
   float m = -INFINITY, l = 0.f;
-  if (tid < splits) {
+  if (tid < used) {
     m = part_ml[(bh * splits + tid) * 2];
     l = part_ml[(bh * splits + tid) * 2 + 1];
   }
@@ -865,14 +893,14 @@ many_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
   __syncthreads();
   const float top = fmaxf(fmaxf(waves[0][0], waves[1][0]), fmaxf(waves[2][0], waves[3][0]));
   const float f = exp2_fast(m - (top == -INFINITY ? 0.f : top));
-  if (tid < splits) weight[tid] = l == 0.f ? -1.f : f;
+  if (tid < used) weight[tid] = l == 0.f ? -1.f : f;
   const float wl = wave_sum(l == 0.f ? 0.f : l * f);
   if (lane == 0) waves[w][1] = wl;
   __syncthreads();
   floatx4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < kMost; ++i) {
-    const float x = row + i * kRows < splits ? weight[row + i * kRows] : -1.f;
+    const float x = row + i * kRows < used ? weight[row + i * kRows] : -1.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] += x < 0.f ? 0.f : x * o[i][e];
   }
@@ -969,6 +997,13 @@ extern "C" int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_str
   return launch_status("pd_select_blocks");
 }
 
+// The next power of two: what a batch's plan depends on.
+int64_t batch_bucket(int32_t batch) {
+  int64_t rows = 1;
+  while (rows < batch) rows *= 2;
+  return rows;
+}
+
 extern "C" int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_heads,
                                int32_t head_dim, int32_t cache_type, int32_t entries,
                                int32_t listed, int32_t cus, int32_t* splits) {
@@ -978,18 +1013,19 @@ extern "C" int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_
     return pd::fail(PD_EINVAL, "batch, heads, entries and CUs must be positive");
   if (!pd::valid_head_dim(head_dim) || !pd::valid_cache(cache_type))
     return pd::fail(PD_EINVAL, "unknown head_dim or cache type");
-  int64_t rows = 1;
-  while (rows < batch) rows *= 2;
-  rows *= int64_t(num_kv_heads) * ((num_heads / num_kv_heads + 15) / 16);
+  const int64_t rows =
+      batch_bucket(batch) * num_kv_heads * ((num_heads / num_kv_heads + 15) / 16);
   // Listed blocks are about as many for every row: one workgroup a CU, each with the most to
   // do behind its start of some 3 us (17 rows of 37 blocks, Hq 32 / Hkv 4 / D 256, e4m3: 22.6
   // us; 28.5 with eight).  Whole caches differ in length: eight a CU, so that no long one is
-  // left to a few (64 of 1 to 32768 tokens, Hq 32 / Hkv 8 / D 128: 404 us; 604 with two; 8 of
-  // 1000 to 9000: 24.5 and 25.1).  Nor is a long list: 128 tiles a workgroup at most.
+  // left to a few (64 of 1 to 32768 tokens, Hq 32 / Hkv 8 / D 128: 387 us; 604 with two; 8 of
+  // 1000 to 9000: 23 and 25).  Nor is a long list or table: 128 tiles a workgroup at most,
+  // while the splits that short sequences leave empty are few enough (32768 workgroups).
   const int64_t groups = int64_t(listed ? 1 : 8) * cus;
   const int64_t tiles = int64_t(entries) * (kBlock / tile_tokens(head_dim, cache_type));
   const int64_t want = std::max((groups + rows - 1) / rows, tiles / 128);
-  const int64_t most = std::min<int64_t>((tiles + 3) / 4, kMaxSplits);
+  const int64_t most =
+      std::min<int64_t>({(tiles + 3) / 4, kMaxSplits, std::max<int64_t>(1, 32768 / rows)});
   *splits = int32_t(std::max<int64_t>(1, std::min(want, most)));
   return PD_OK;
 }
@@ -1020,6 +1056,10 @@ extern "C" int pd_block_decode(const void* q, int64_t q_stride_b, int64_t q_stri
   p.out = u16(out), p.qsb = q_stride_b, p.qsh = q_stride_h;
   p.group = num_heads / num_kv_heads, p.tiles = (p.group + 15) / 16;
   p.scale2 = float(scale * 1.4426950408889634);
+  // With more workgroups than the device holds, a workgroup's start is worth another tile: 64
+  // sequences of 500 to 1500 tokens with room for 32768 take 38.3 us with one, 37.6 with two,
+  // 40.1 with four, 8 of 1000 to 9000 24.5, 23.0 and 23.7.
+  p.two = batch_bucket(batch) * num_kv_heads * p.tiles * splits > 2048;
   const int64_t columns = int64_t(num_kv_heads) * p.tiles;
   if (batch > 65535 || columns * splits * batch > 0x7fffffff)
     return pd::fail(PD_EINVAL, "grid dimension exceeds device limits");
@@ -1042,18 +1082,20 @@ extern "C" int pd_block_decode(const void* q, int64_t q_stride_b, int64_t q_stri
   if (!fits) return pd::fail(PD_ELAUNCH, "pd_block_decode: LDS size");
   if (const int bad = launch_status("pd_block_decode")) return bad;
   if (splits == 1) return PD_OK;
+  const int tile = tile_tokens(head_dim, cache_type);
+  const SplitRule rule{table_width, blocks ? kBlock / tile * kept : 0, tile, p.two, splits};
   if (splits <= kFewSplits) {
     const int64_t total = int64_t(batch) * num_heads * head_dim;
     const auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(unsigned((total + 1023) / 1024)), dim3(256), 0,
-                         as_stream(stream), part_o, part_ml, p.out, splits, head_dim, total,
+                         as_stream(stream), part_o, part_ml, p.out, lengths, rule, head_dim, total,
                          v_scale, p.group, num_heads);
     };
     go(splits <= 2 ? few_merge_kernel<2> : splits <= 4 ? few_merge_kernel<4> : few_merge_kernel<8>);
   } else {
     const auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(unsigned(batch * num_heads), head_dim / kMergeCols),
-                         dim3(256), 0, as_stream(stream), part_o, part_ml, p.out, splits, head_dim,
+                         dim3(256), 0, as_stream(stream), part_o, part_ml, p.out, lengths, rule, head_dim,
                          v_scale, p.group, num_heads);
     };
     go(splits <= 16   ? many_merge_kernel<1>
