@@ -9,6 +9,27 @@
 //                      listed blocks, or over all of them
 //
 // A block is 64 tokens, a quarter of a page.
+//
+// Attention: bound by the bytes of K and V.  Wavefronts walk the tiles of a
+// sequence (or list) with private softmax states, K and V in registers from
+// their loads to the matrix instructions, and are joined in LDS at the end of a
+// workgroup; the splits of a sequence by a second launch.  Matrix and vector
+// instructions take a quarter of the time that the bytes do (counters: 64
+// sequences of up to 32768 e4m3 tokens, Hq 32 / Hkv 8 / D 128, 24% of the SIMDs'
+// clocks), which is what the products in two bf16 terms of the probabilities and
+// the e4m3 conversions are paid from.  Measured on MI355X, both launches:
+//   64 sequences of 1 to 32768 e4m3 tokens, Hq 32 / Hkv 8 / D 128   388 us  5.5 TB/s
+//   128 of 1 to 4096, Hq = Hkv = 16, D 64                           124 us  4.5 TB/s
+//   64 sequences, 64 listed bf16 blocks, Hq 32 / Hkv 8 / D 128      177 us  5.5 TB/s
+//   17 sequences, 37 listed e4m3 blocks, Hq 32 / Hkv 4 / D 256     22.6 us  3.5 TB/s
+//   one, 64 listed bf16 blocks, Hq 16 / Hkv 4 / D 256               9.6 us, launches and
+//   one of 2064 e4m3 tokens, the same heads                         8.3 us  latencies
+// (a copy of 2 GiB reads and writes 4.85 TB/s).  Of the last two 6 us are the
+// attention's chain: length, table, K, softmax, join, write.
+//
+// Selection: the scores are bound by their double-precision arithmetic (60% of
+// the SIMDs' clocks where the bounds' bytes would take 14 us: 64 sequences of up
+// to 32768 tokens, 21 us), the choice by its barriers (4 to 7 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -42,6 +63,10 @@ __device__ __forceinline__ int block_count(const int32_t* lengths, int b, int wi
 // Scores are sums of exact products in 64 bits, so the order of a sum moves no
 // block: two implementations pick the same ones unless their scores agree to 15
 // digits without being equal.
+//
+// Two launches: one workgroup for a (sequence, kv head), with its keys in LDS, is
+// 7.7 instead of 10.3 us for 16 sequences of up to 16384 tokens of 16 kv heads,
+// and 31 instead of 8 for one sequence of 32768 of 4.
 struct SelectArgs {
   const int32_t *lengths, *table;
   const uint16_t *q, *bounds;
@@ -457,7 +482,13 @@ struct DecodeArgs {
 // of a channel in a lane: a lane loads kRun channels of eight tokens and turns the 8 x kRun
 // square with byte permutes; row m of the MFMA of channel j is channel kRun m + j.  No value
 // crosses a lane or the LDS before the end.  A bf16 tile at head_dim 256 is 16 tokens, its
-// P V MFMAs 16 x 16 x 16.
+// P V MFMAs 16 x 16 x 16: 32 tokens did not fit two wavefronts a SIMD without spills (32
+// sequences of 64 blocks, Hq 16 / Hkv 4: 110 us, 94 with 16).
+//
+// Tiles of 64 e4m3 tokens: 26.7 instead of 23.5 us for 8 sequences of 1000 to 9000 (Hkv 8, D
+// 128), 38.5 and 35 for 16 (Hkv 16, D 64), 408 and 415 for 64 of up to 32768; of 32 bf16
+// tokens at D 64: 107 instead of 93 for 64 sequences of 32 blocks.  A second tile on its way
+// is no faster at D 64 and slower at D 128 (455 instead of 388), where it costs a wavefront.
 template <int D, bool kE4m3>
 struct Decode {
   static constexpr int kBytes = kE4m3 ? 1 : 2;
@@ -487,8 +518,9 @@ struct Words {
   uint32_t w[N];
 };
 
-// Rows of 512 bytes pass the caches by; the lines of shorter ones are still to be read by
-// another load.
+// Rows of 512 bytes pass the caches by (32 sequences of 64 blocks: 94 -> 87 us); the lines of
+// shorter ones are still to be read by another load (64 e4m3 sequences of 128-byte rows: 394
+// -> 511).
 template <typename V, int kRowBytes>
 __device__ __forceinline__ V load_row(const char* p) {
   if constexpr (kRowBytes >= 512)

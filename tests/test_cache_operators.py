@@ -130,3 +130,28 @@ def test_plain_forms_on_small_cases():
     out, _ = O.attention(q, k, v, torch.zeros((1, 1), dtype=torch.int32), torch.tensor([65]),
                          torch.tensor([[[1, 1, 0]]]))
     assert out[0, 0, 0] == pytest.approx(6 / 66)
+
+
+def test_a_launch_runs_on_the_device_of_its_tensors(monkeypatch):
+    seen, inside = [], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            inside.append(self.index)
+
+        def __exit__(self, *error):
+            inside.pop()
+
+    def function(*args):
+        seen.append((args, tuple(inside)))
+        return _native.PD_OK
+
+    monkeypatch.setattr(_native, "_current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_native, "_raw_stream", lambda index: 100 + index)
+    _native.launch(0, function, 7)
+    _native.launch(1, function, 8)
+    assert seen == [((7, 100), ()), ((8, 101), (1,))]

@@ -291,3 +291,26 @@ def test_refused_tensors():
         call(dict(x, k=x["k"].clone().requires_grad_()))
     with pytest.raises(ValueError, match="multiple of 8"):
         call(dict(x, rope=x["rope"][:, :12].contiguous()))
+
+
+def test_quotients_at_the_midpoints_of_e4m3():
+    """The stored value is the rounded division's: products of a scale with the midpoints and
+    values of e4m3, and the floats next to them, through a rotation by (cos, 0)."""
+    n, d = 512, 64
+    rng = np.random.default_rng(33)
+    grid = torch.arange(127, dtype=torch.uint8).view(E4M3).float()
+    grid = torch.cat([grid, (grid[1:] + grid[:-1]) / 2])
+    scale = torch.tensor([0.0123, 3.0, 1e-6, 7.7e8], dtype=torch.float32)
+    pick = grid[torch.from_numpy(rng.integers(0, len(grid), (4, n, d // 2)))]
+    near = torch.from_numpy(rng.integers(-2, 3, (4, n, d // 2)).astype(np.int32))
+    for h in range(4):                 # one scale at a time, as every head's keys are one
+        x = pick[h] * scale[h]
+        x = (x.view(torch.int32) + near[h] * (x > 0)).view(torch.float32)
+        rope = torch.stack([x, torch.zeros_like(x)], -1).cuda()              # [n, d / 2, 2]
+        ones = torch.cat([torch.ones(n, 1, d // 2), torch.zeros(n, 1, d // 2)], 2)
+        k = ones.bfloat16().cuda()
+        cache = [torch.zeros((2, 256, 1, d), device="cuda").to(E4M3) for _ in range(2)]
+        at = torch.arange(n, device="cuda")
+        append_kv(None, k, k, at, rope, *cache, at.int(), k_scale=scale[h:h + 1].cuda())
+        want = O.stored(x[:, None], scale[h:h + 1], E4M3)
+        assert torch.equal(bits(cache[0]).view(n, d)[:, :d // 2], bits(want)[:, 0])

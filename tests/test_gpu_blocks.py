@@ -232,12 +232,14 @@ def test_strided_queries_narrow_tables_and_part_batches(kind):
     blocks = random_blocks(x, 9, seed=41)
     res = allocate_block_resources(DecodeSpec(5, 8, 2, 128, 4096), "cuda", kept=9)
     res.out.fill_(7.0)
+    res.blocks.fill_(-9)
     out = attend(x, g, res, blocks.cuda())
     check(out, x, blocks)
     assert (res.out[3:] == 7.0).all()
     bounds = bounds_of(x, 41)
     got = select_blocks(g["q"], bounds.cuda(), g["tables"], g["lengths"], resources=res)
     assert torch.equal(got.cpu(), O.select(x["q"], bounds, x["tables"], x["lengths"], 9))
+    assert (res.blocks[3:] == -9).all()
 
 
 @pytest.mark.parametrize("kind", KINDS, ids=IDS)
