@@ -474,8 +474,8 @@ int pd_block_bounds(const void* k_cache, int32_t cache_type, int64_t num_slots,
  * first `first` and last `last` (at least 1: a block that is not full has no
  * bounds) and those of the highest scores, score = max over the group's query
  * heads of sum_d max(q, 0) high + min(q, 0) low in 64 bits, ties to the lowest
- * block; ascending, -1 behind a sequence of fewer.  A NaN score counts as
- * +infinity, a page outside [0, num_pages) as the lowest.  keys: workspace uint64
+ * block; ascending, -1 behind a sequence of fewer.  A NaN score (an infinite
+ * query's too) counts as +infinity, a page outside [0, num_pages) as the lowest.  keys: workspace uint64
  * [batch, Hkv, table_width * 4]. */
 int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* bounds,
                      int64_t num_pages, const int32_t* table, int64_t table_stride_b,

@@ -38,6 +38,7 @@ def block_bounds(keys):
 def scores(q, bounds):
     """float64 [blocks] of q [G, D] and bounds [blocks, 2, D]."""
     q, bounds = q.double(), bounds.double()
+    q = torch.where(q.isinf(), math.nan, q)
     each = q.clamp(min=0) @ bounds[:, 1].T + q.clamp(max=0) @ bounds[:, 0].T      # [G, blocks]
     return torch.where(each.isnan(), math.inf, each).amax(0)
 

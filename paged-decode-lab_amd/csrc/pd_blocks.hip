@@ -107,8 +107,9 @@ struct Query {
       const int64_t head = int64_t(g) * p.group + min(head0 + h, p.group - 1);
       float f[8];
       unpack8(load16(p.q + b * p.qsb + head * p.qsh + 8 * part), f);
+      // f - f: an infinity becomes a NaN, with which every score is one.
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[h][i] = f[i];
+      for (int i = 0; i < 8; ++i) x[h][i] = f[i] + (f[i] - f[i]);
     }
   }
 };
@@ -131,7 +132,7 @@ struct Bounds {
 
 // max(q, 0) hi + min(q, 0) lo = q (hi + lo) / 2 + |q| (hi - lo) / 2, whose factors one
 // conversion of q serves; the halves are left out, they move no order.  (An infinite bound
-// gives the same infinity or NaN in both.)  The largest of kHeads heads' sums, in every
+// gives the same infinity or NaN in both, for a finite q.)  The largest of kHeads heads' sums, in every
 // lane of the block: a lane pair splits the heads between them at each of the first steps,
 // so that a step moves half of the sums of the one before.
 template <int D, int kHeads>
@@ -749,12 +750,14 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
 #pragma unroll
       for (int a = 0; a < T::kGroups; ++a) {
         // p = hi + lo to 16 significant bits: bf16 probabilities alone would add an
-        // error as large as the output's own rounding.
+        // error as large as the output's own rounding.  hi is below p, so that lo is not
+        // zero where p is not: an infinite V times either is that infinity.
         Words<T::kPer / 2> hi, lo;
 #pragma unroll
         for (int i = 0; i < T::kPer / 2; ++i) {
           const float x0 = x[a][2 * i], x1 = x[a][2 * i + 1];
-          const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
+          const uint32_t b0 = __builtin_elementwise_sub_sat(__float_as_uint(x0), 1u);
+          const uint32_t b1 = __builtin_elementwise_sub_sat(__float_as_uint(x1), 1u);
           hi.w[i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
           lo.w[i] = pack_bf16(x0 - __uint_as_float(b0 & 0xffff0000u),
                               x1 - __uint_as_float(b1 & 0xffff0000u));
@@ -1093,7 +1096,8 @@ extern "C" int pd_block_decode(const void* q, int64_t q_stride_b, int64_t q_stri
   // 40.1 with four, 8 of 1000 to 9000 24.5, 23.0 and 23.7.
   p.two = batch_bucket(batch) * num_kv_heads * p.tiles * splits > 2048;
   const int64_t columns = int64_t(num_kv_heads) * p.tiles;
-  if (batch > 65535 || columns * splits * batch > 0x7fffffff)
+  if (batch > 65535 || columns * splits * batch > 0x7fffffff ||
+      int64_t(batch) * num_heads > 0x7fffffff)
     return pd::fail(PD_EINVAL, "grid dimension exceeds device limits");
   const dim3 grid = {unsigned(columns), unsigned(splits), unsigned(batch)};
   const unsigned lds = unsigned(128 + 4 * (p.group < 16 ? p.group : 16) * head_dim) * 4;

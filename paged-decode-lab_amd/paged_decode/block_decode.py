@@ -150,8 +150,8 @@ def select_blocks(q, bounds, tables, lengths, *, resources, first=1, last=1):
     in; the others by score, the largest of the group's query heads' sums over the channels of
     max(q, 0) high + min(q, 0) low, computed in 64 bits; ties go to the lowest block.
     ``bounds`` as of ``kv_append``, of the keys as they are stored (a scale per kv head moves
-    no block).  ``last`` is at least 1: the block being filled has no bounds.  A NaN score
-    counts as infinite."""
+    no block).  ``last`` is at least 1: the block being filled has no bounds.  A NaN score, an
+    infinite query's too, counts as infinite."""
     batch, device, stride_b, stride_h, table_stride, width = _check_step(q, tables, lengths,
                                                                          resources)
     spec, blocks = resources.spec, resources.blocks

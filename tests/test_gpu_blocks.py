@@ -147,6 +147,21 @@ def test_infinite_and_nan_keys_and_values_stay_in_their_rows():
     assert out[~odd].isfinite().all()
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_an_infinite_value_of_probability_one(d):
+    """Probabilities that a bf16 holds exactly: one, and a half and a quarter of equal scores."""
+    x = make([1, 2, 4], 4, 1, d, torch.bfloat16, seed=25)
+    for b in range(3):
+        x["k"][int(x["tables"][b, 0])] = 0.0
+        x["v"][int(x["tables"][b, 0]), 0, 0, 1] = float("inf")
+        x["v"][int(x["tables"][b, 0]), 0, 0, d - 1] = -float("inf")
+    g = dev(x)
+    blocks = torch.zeros((3, 1, 1), dtype=torch.int32)
+    out = attend(x, g, allocate_block_resources(spec_of(x), "cuda", kept=1), blocks.cuda()).cpu()
+    assert (out[..., 1] == float("inf")).all() and (out[..., d - 1] == -float("inf")).all()
+    assert out[..., 2:d - 1].isfinite().all() and out[..., 0].isfinite().all()
+
+
 def test_scores_of_large_magnitude():
     """Maxima far from zero and far apart: the running maximum moves at every tile."""
     x = make([900, 900], 4, 1, 128, torch.bfloat16, seed=24)
@@ -197,12 +212,13 @@ def test_select_odd_scores():
     bounds[at(0, 9)][0, 1] = float("inf")
     x["q"][1] = 0.0                                   # every score equal: the first blocks
     x["q"][2, 0, 0] = float("nan")                    # every score of kv head 0 infinite
+    x["q"][2, 3, 9] = -float("inf")                   # and of kv head 1
     res = allocate_block_resources(spec_of(x), "cuda", kept=6)
     got = select_blocks(x["q"].cuda(), bounds.cuda(), x["tables"].cuda(), x["lengths"].cuda(),
                         resources=res).cpu()
     assert torch.equal(got, O.select(x["q"], bounds, x["tables"], x["lengths"], 6))
     assert {9, 30} <= set(got[0, 0].tolist()) and 7 in got[0, 1].tolist()
-    assert got[1, 0].tolist() == [0, 1, 2, 3, 4, 46] == got[2, 0].tolist()
+    assert got[1, 0].tolist() == [0, 1, 2, 3, 4, 46] == got[2, 0].tolist() == got[2, 1].tolist()
 
 
 def test_select_from_a_long_table():
