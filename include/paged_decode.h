@@ -451,9 +451,9 @@ int pd_delta_step(const float* act, const void* a, const void* b, const void* a_
  * half) or, interleaved, (2j, 2j + 1); half 0: no rotation, positions and rope
  * may be null.  q [rows, Hq, D] -> q_out (may be q); key and value -> slot
  * slot_mapping[i] of the caches, in an e4m3 cache as round(clamp(x / scale,
- * +-448)).  A slot outside [0, num_slots) skips the write; a position outside
- * the table too, and the rotated part of its query is NaN.  Slots of one call
- * must differ.  Row strides are in elements, multiples of 8, heads contiguous;
+ * +-448)), scales positive normal numbers.  A slot outside [0, num_slots) skips
+ * the write; a position outside the table too, and the rotated part of its query
+ * is NaN.  Slots of one call must differ.  Row strides are in elements, multiples of 8, heads contiguous;
  * half is a multiple of 8; num_heads may be 0.  bounds (may be null): as
  * pd_block_bounds, of the keys just written. */
 int pd_append_kv(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,

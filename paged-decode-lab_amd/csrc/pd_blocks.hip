@@ -132,9 +132,9 @@ struct Bounds {
 
 // max(q, 0) hi + min(q, 0) lo = q (hi + lo) / 2 + |q| (hi - lo) / 2, whose factors one
 // conversion of q serves; the halves are left out, they move no order.  (An infinite bound
-// gives the same infinity or NaN in both, for a finite q.)  The largest of kHeads heads' sums, in every
-// lane of the block: a lane pair splits the heads between them at each of the first steps,
-// so that a step moves half of the sums of the one before.
+// gives the same infinity or NaN in both, for a finite q.)  The largest of kHeads heads' sums,
+// in every lane of the block: a lane pair splits the heads between them at each of the first
+// steps, so that a step moves half of the sums of the one before.
 template <int D, int kHeads>
 __device__ __forceinline__ double best_of(const Query<D, kHeads>& q, const double (&mid)[8],
                                           const double (&radius)[8], int lane) {
@@ -364,7 +364,7 @@ __device__ __forceinline__ void pick_blocks(Picker<kWaves>& t, const uint64_t* _
 
   for (int j = tid; j < begin; j += kThreads) out[j] = j;
   for (int i = tid; i < n - end; i += kThreads) out[begin + taken + i] = end + i;
-  // In order: kWave threads' blocks at a time, a thread's place by the counts ahead of it.
+  // In order: a block a thread at a time, a thread's place by the counts ahead of it.
   const uint64_t below = (uint64_t(1) << lane) - 1;
   uint32_t written = begin, ties = 0;
   const auto marks = [&](int j, uint64_t key, bool& in, bool& tie) {

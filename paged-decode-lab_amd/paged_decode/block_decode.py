@@ -12,6 +12,7 @@ are not checked, nothing allocates, synchronizes or reads device memory on the h
 can be captured in a hipGraph).  Lengths past the table count as its capacity; a page outside
 the cache is read as having no tokens.  A sequence's output depends on the batch through its
 next power of two alone, so a padded graph bucket gives the bits of the eager call.
+Inference only.
 """
 from dataclasses import dataclass, field
 import math

@@ -97,9 +97,10 @@ def append_kv(q, k, v, positions, rope, k_cache, v_cache, slot_mapping, *, inter
     ``positions`` int64 [N]: element pairs (j, j + half), or (2j, 2j + 1) with ``interleaved``,
     of the leading 2 half elements are rotated, half a multiple of 8; rope None rotates nothing.
     Caches [blocks, block_size, Hkv, D] bf16 or float8_e4m3fn, which holds x / scale (scales
-    positive, float32 [Hkv], None: 1), clamped to +-448; ``slot_mapping`` int32 [N], a negative slot (or one past the cache) writes
-    nothing, slots of one call must differ.  A position outside the table writes nothing and
-    gives its query NaN.  ``out``: where the queries go (q itself: in place).
+    positive normal numbers, float32 [Hkv], None: 1), clamped to +-448; ``slot_mapping`` int32
+    [N], a negative slot (or one past the cache) writes nothing, slots of one call must differ.
+    A position outside the table writes nothing and gives its query NaN.  ``out``: where the
+    queries go (q itself: in place).
     """
     shape, device = k.shape, k.get_device()
     if len(shape) != 3 or device < 0:
@@ -134,6 +135,8 @@ def append_kv(q, k, v, positions, rope, k_cache, v_cache, slot_mapping, *, inter
         if (len(form) != 3 or form[2] != 2 or rope.dtype != torch.float32
                 or not rope.is_contiguous() or rope.get_device() != device):
             _refuse("rope must be contiguous float32 [positions, half, 2] on the key's device")
+        if positions is None:
+            _refuse("rope needs positions")
         _check_index(positions, n, torch.int64, device, "positions")
         table = (positions.data_ptr(), rope.data_ptr(), form[0], form[1])
     heads = q_stride = out_stride = 0

@@ -291,6 +291,8 @@ def test_refused_tensors():
         call(dict(x, k=x["k"].clone().requires_grad_()))
     with pytest.raises(ValueError, match="multiple of 8"):
         call(dict(x, rope=x["rope"][:, :12].contiguous()))
+    with pytest.raises(ValueError, match="needs positions"):
+        call(dict(x, positions=None))
 
 
 def test_quotients_at_the_midpoints_of_e4m3():
