@@ -214,22 +214,21 @@ def _decode_inputs(case, seed):
 
 
 def _package():
-    """The package's modules of the decode operators and the geometry, and append_kv."""
+    """The package's modules of these operators."""
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                         "paged-decode-lab_amd")
     if root not in sys.path:
         sys.path.insert(0, root)
     from paged_decode import block_decode, kv_append, spec
-    return block_decode, kv_append.append_kv, spec
+    return block_decode, kv_append, spec
 
 
 def prepare(case, seed):
-    make = _append_inputs if case["kind"] == "append" else _decode_inputs
-    state = dict(case=case, **make(case, seed))
+    if case["kind"] == "append":
+        return dict(case=case, **_append_inputs(case, seed))
+    state = dict(case=case, **_decode_inputs(case, seed))
     if own:
-        block_decode, state["append_kv"], spec = _package()
-        state["block_decode"] = block_decode
-    if own and case["kind"] != "append":
+        block_decode, _, spec = _package()
         geometry = spec.DecodeSpec(case["batch"], case["hq"], case["hkv"], case["dim"],
                                    case["high"])
         state["resources"] = block_decode.allocate_block_resources(geometry, DEV,
@@ -242,12 +241,13 @@ def run(state):
     if not own:
         return {"append": _plain_append, "fp8": _plain_fp8, "select": _plain_select,
                 "sparse": _plain_sparse}[kind](state)
-    block_decode = state["block_decode"]
+    block_decode, kv_append, _ = _package()
     if kind == "append":
-        q = state["append_kv"](state["q"], state["k"], state["v"], state["positions"],
-                               state["rope"], state["k_cache"], state["v_cache"], state["slots"],
-                               interleaved=case["interleaved"], k_scale=state["k_scale"],
-                               v_scale=state["v_scale"], bounds=state["bounds"])
+        q = kv_append.append_kv(state["q"], state["k"], state["v"], state["positions"],
+                                state["rope"], state["k_cache"], state["v_cache"],
+                                state["slots"], interleaved=case["interleaved"],
+                                k_scale=state["k_scale"], v_scale=state["v_scale"],
+                                bounds=state["bounds"])
         return {"q": q, "k_cache": state["k_cache"], "v_cache": state["v_cache"],
                 "bounds": state["bounds"]}
     if kind == "fp8":
