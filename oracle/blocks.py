@@ -69,8 +69,7 @@ def attention(q, k, v, tables, lengths, blocks=None, scale=None, k_scale=None, v
     * a score is a float32 sum of D exact products: (D + 2) 2^-24 sum |q k|, and its product
       with the scales two more roundings; a probability's relative error is that times the
       scale, twice (its own and the maximum's), and 2^-22 of the exponential;
-    * the probability is taken to 16 significant bits (2^-15), and the sums over n tokens add
-      n 2^-24 each, numerator and denominator.
+    * the sums over n tokens add n 2^-24 each, numerator and denominator.
     """
     batch, heads, dim = q.shape
     hkv = k.shape[2]
@@ -100,7 +99,7 @@ def attention(q, k, v, tables, lengths, blocks=None, scale=None, k_scale=None, v
             out[b, at] = p @ values * by
             spread = ((dim + 4) * 2.0 ** -24 * abs(factor)
                       * (rows.abs() @ keys.abs().T).amax(-1, keepdim=True))
-            relative = 2 * spread + 2.0 ** -15 + 2.0 ** -21 + 2 * (len(tokens) + 64) * 2.0 ** -24
+            relative = 2 * spread + 2.0 ** -21 + 2 * (len(tokens) + 64) * 2.0 ** -24
             bound[b, at] = relative * (p @ values.abs() * abs(by))
     return out, bound
 

@@ -16,8 +16,8 @@
 // workgroup; the splits of a sequence by a second launch.  Matrix and vector
 // instructions take a quarter of the time that the bytes do (counters: 64
 // sequences of up to 32768 e4m3 tokens, Hq 32 / Hkv 8 / D 128, 24% of the SIMDs'
-// clocks), which is what the products in two bf16 terms of the probabilities and
-// the e4m3 conversions are paid from.  Measured on MI355X, both launches:
+// clocks), which is what the products in three bf16 terms of the probabilities
+// and the e4m3 conversions are paid from.  Measured on MI355X, both launches:
 //   64 sequences of 1 to 32768 e4m3 tokens, Hq 32 / Hkv 8 / D 128   388 us  5.5 TB/s
 //   128 of 1 to 4096, Hq = Hkv = 16, D 64                           124 us  4.5 TB/s
 //   64 sequences, 64 listed bf16 blocks, Hq 32 / Hkv 8 / D 128      177 us  5.5 TB/s
@@ -565,6 +565,23 @@ __device__ __forceinline__ floatx4_t mfma_pv(const Words<kPer / 2>& a, const Wor
                                                      __builtin_bit_cast(short4v_t, b), c, 0, 0, 0);
 }
 
+// A probability as three bf16, in the upper halves of the words: 8 bits each of its 24, by
+// cutting.  One term's error would be as large as the output's own rounding; two (16 bits) move
+// some outputs to the other side of theirs (64 sequences of up to 32768 e4m3 tokens: 1.3e-4
+// from the float32 form, relative, 2.2e-5 with three) and are hardly cheaper (398 us both; 16
+// of up to 8192, Hkv 16, D 64: 34.3 and 35.5).  Where p is not zero, neither is any of them (2^-133 at least), so that an infinite
+// V times each is that infinity: 2^-132 more than p at most, which float32 does not see for p
+// above 2^-108.
+struct Terms {
+  uint32_t hi, mid, lo;
+  __device__ __forceinline__ explicit Terms(float p) {
+    hi = __float_as_uint(p);
+    const uint32_t least = min(hi, 0x10000u);
+    mid = max(__float_as_uint(p - __uint_as_float(hi & 0xffff0000u)), least);
+    lo = max(__float_as_uint(__uint_as_float(mid) - __uint_as_float(mid & 0xffff0000u)), least);
+  }
+};
+
 template <int D, bool kE4m3>
 struct Tile {
   using T = Decode<D, kE4m3>;
@@ -749,25 +766,25 @@ block_decode_kernel(const int32_t* __restrict__ lengths, const int32_t* __restri
       }
 #pragma unroll
       for (int a = 0; a < T::kGroups; ++a) {
-        // p = hi + lo to 16 significant bits: bf16 probabilities alone would add an
-        // error as large as the output's own rounding.  hi is below p, so that lo is not
-        // zero where p is not: an infinite V times either is that infinity.
-        Words<T::kPer / 2> hi, lo;
+        // p = hi + mid + lo, each a bf16: all 24 bits of p.
+        Words<T::kPer / 2> hi, mid, lo;
 #pragma unroll
         for (int i = 0; i < T::kPer / 2; ++i) {
-          const float x0 = x[a][2 * i], x1 = x[a][2 * i + 1];
-          const uint32_t b0 = __builtin_elementwise_sub_sat(__float_as_uint(x0), 1u);
-          const uint32_t b1 = __builtin_elementwise_sub_sat(__float_as_uint(x1), 1u);
-          hi.w[i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-          lo.w[i] = pack_bf16(x0 - __uint_as_float(b0 & 0xffff0000u),
-                              x1 - __uint_as_float(b1 & 0xffff0000u));
+          const Terms x0(x[a][2 * i]), x1(x[a][2 * i + 1]);
+          hi.w[i] = __builtin_amdgcn_perm(x1.hi, x0.hi, 0x07060302u);
+          mid.w[i] = __builtin_amdgcn_perm(x1.mid, x0.mid, 0x07060302u);
+          lo.w[i] = __builtin_amdgcn_perm(x1.lo, x0.lo, 0x07060302u);
         }
+        // All words before the first product: 2 to 18 registers fewer (bf16, D 128: no spill,
+        // 8 lists of 32 blocks 14.8 instead of 15.4 us).
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int c = 0; c < T::kChunks; ++c)
 #pragma unroll
           for (int j = 0; j < T::kRun; ++j) {
             const Words<T::kPer / 2> operand = t.v_operand(a, c, j);
             o[c * T::kRun + j] = mfma_pv<T::kPer>(operand, lo, o[c * T::kRun + j]);
+            o[c * T::kRun + j] = mfma_pv<T::kPer>(operand, mid, o[c * T::kRun + j]);
             o[c * T::kRun + j] = mfma_pv<T::kPer>(operand, hi, o[c * T::kRun + j]);
           }
       }

@@ -1,0 +1,89 @@
+"""The cache operators where their arithmetic or their arguments are at an edge: weights that
+cancel, bounds of any width, scales at the ends of float32, strides of a single row."""
+import math
+
+import pytest
+import torch
+
+if not torch.cuda.is_available():
+    pytest.skip("needs an MI355X GPU", allow_module_level=True)
+
+from oracle import blocks as O
+from paged_decode.block_decode import allocate_block_resources, fp8_decode, sparse_decode
+from paged_decode.spec import DecodeSpec
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+KINDS = [torch.bfloat16, E4M3]
+IDS = ["bf16", "e4m3"]
+
+
+def two_tokens(scores, values, dim, kind, scale, heads=4):
+    """Attention over two tokens a sequence: scores [B, 2], held exactly by `kind` and times
+    `scale`, values [B, 2, D]."""
+    batch = len(scores)
+    k, v = torch.zeros((batch, 256, 1, dim)), torch.zeros((batch, 256, 1, dim))
+    k[:, :2, 0, 1], v[:, :2, 0] = scores, values
+    k, v = (t.to(kind).cuda() for t in (k, v))
+    assert torch.equal(k[:, :2, 0, 1].float().cpu(), scores)
+    q = torch.zeros((batch, heads, dim), dtype=torch.bfloat16, device="cuda")
+    q[..., 1] = 1.0
+    tables = torch.arange(batch, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    lengths = torch.full((batch,), 2, dtype=torch.int32, device="cuda")
+    spec = DecodeSpec(batch, heads, 1, dim, 256)
+    if kind == E4M3:
+        return fp8_decode(q, k, v, tables, lengths, scale=scale,
+                          resources=allocate_block_resources(spec, "cuda")).cpu()
+    blocks = torch.zeros((batch, 1, 1), dtype=torch.int32, device="cuda")
+    return sparse_decode(q, k, v, tables, lengths, blocks, scale=scale,
+                         resources=allocate_block_resources(spec, "cuda", kept=1)).cpu()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_weights_that_cancel(dim, kind):
+    """Two tokens of values 1 and -1 whose weights differ by 2^-13 to 2^-10 of themselves: the
+    output (1 - p) / (1 + p) is as exact as the weights.
+
+    Float32: p = 2^x, x = -score scale log2 e below 2^-9 in size, so that its roundings move p by
+    2^-32 and the exponential by 2^-22; the numerator's sum has up to four additions of numbers
+    up to 1, 2^-23 each where an instruction truncates.  (2^-22 + 2^-21) / (1 + p) is below 2^-21,
+    the quotient's own rounding 2^-23 of it; then the output's half step, 2^-8 of it."""
+    sizes = torch.arange(8, 16) / 8.0                       # 1 to 1.875: exact in e4m3
+    scores = torch.stack([torch.zeros(8), -sizes], 1)
+    values = torch.tensor([1.0, -1.0])[None, :, None].expand(8, 2, dim)
+    for i in range(24):
+        scale = 2.0 ** -13 * (1 + i / 7)
+        p = torch.exp(-sizes.double() * scale)
+        exact = ((1 - p) / (1 + p))[:, None, None]
+        got = two_tokens(scores, values, dim, kind, scale).double()
+        allowed = 2.0 ** -21 + 2.0 ** -8 * (exact + 2.0 ** -21)
+        error = (got - exact).abs()
+        assert (error <= allowed).all(), (i, float((error / allowed).max()))
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_infinite_and_huge_values_of_small_weights(dim, kind):
+    """A weight of 2^-x: an infinite value (bf16 alone holds one) makes its channel infinite,
+    the largest finite one adds what it is worth, and nothing once the weight is zero."""
+    steps = [0.0, 8, 24, 30, 60, 88, 96, 104, 120, 160, 448]
+    scores = torch.tensor([[0.0, -s] for s in steps])
+    big = 448.0 if kind == E4M3 else float(torch.finfo(torch.bfloat16).max)
+    values = torch.ones((len(steps), 2, dim))
+    values[:, 1, 0] = big
+    values[:, 1, dim - 1] = -big
+    if kind != E4M3:
+        values[:9, 1, 1], values[:9, 1, 2] = math.inf, -math.inf
+    got = two_tokens(scores, values, dim, kind, math.log(2.0)).double()
+    for i, s in enumerate(steps):
+        p = 2.0 ** -s
+        for c, value in ((0, big), (dim - 1, -big), (3, 1.0)):
+            exact = (1 + p * value) / (1 + p)
+            # x = -s: the two roundings of its factor, 2^-23 s; the exponential's 2^-22; sums
+            # and quotient 2^-21.  A weight below 2^-126 is zero.
+            lost = p * abs(value) if s > 120 else 0.0
+            allowed = (2.0 ** -23 * s + 2.0 ** -20) * (1 + p * abs(value)) + lost
+            assert ((got[i, :, c] - exact).abs() <= allowed + 2.0 ** -8 * (abs(exact) + allowed)).all(), (s, c)
+        if kind != E4M3 and i < 9:
+            assert (got[i, :, 1] == math.inf).all() and (got[i, :, 2] == -math.inf).all(), s
