@@ -60,9 +60,11 @@ __device__ __forceinline__ int block_count(const int32_t* lengths, int b, int wi
 
 // ------------------------------------------------------------------ selection
 
-// Scores are sums of exact products in 64 bits, so the order of a sum moves no
-// block: two implementations pick the same ones unless their scores agree to 15
-// digits without being equal.
+// A score takes of each channel the corner that the query's sign asks for and
+// never the other, however large that is.  The products are exact in 64 bits, the
+// sums off by 2^-53 of the taken products' sizes: two implementations pick the
+// same blocks unless scores agree to some 15 digits of their terms without being
+// equal.
 //
 // Two launches: one workgroup for a (sequence, kv head), with its keys in LDS, is
 // 7.7 instead of 10.3 us for 16 sequences of up to 16384 tokens of 16 kv heads,
@@ -130,22 +132,50 @@ struct Bounds {
   }
 };
 
-// max(q, 0) hi + min(q, 0) lo = q (hi + lo) / 2 + |q| (hi - lo) / 2, whose factors one
-// conversion of q serves; the halves are left out, they move no order.  (An infinite bound
-// gives the same infinity or NaN in both, for a finite q.)  The largest of kHeads heads' sums,
-// in every lane of the block: a lane pair splits the heads between them at each of the first
-// steps, so that a step moves half of the sums of the one before.
-template <int D, int kHeads>
-__device__ __forceinline__ double best_of(const Query<D, kHeads>& q, const double (&mid)[8],
-                                          const double (&radius)[8], int lane) {
+// A bf16 as a double is the upper word of it, above a word of zeros.
+__device__ __forceinline__ uint32_t upper(float x) {
+  return uint32_t(__builtin_bit_cast(uint64_t, double(x)) >> 32);
+}
+__device__ __forceinline__ double of_upper(uint32_t w) {
+  return __builtin_bit_cast(double, uint64_t(w) << 32);
+}
+
+// The corners of one block, this lane's channels.
+struct Corners {
+  uint32_t lo[8], hi[8];
+  bool finite;
+  __device__ __forceinline__ Corners(u32x4_t raw_lo, u32x4_t raw_hi) {
+    float l[8], h[8];
+    unpack8(raw_lo, l);
+    unpack8(raw_hi, h);
+    float most = 0.f;  // NaN where one is
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lo[i] = upper(l[i]), hi[i] = upper(h[i]);
+      most = __builtin_elementwise_maximum(
+          __builtin_elementwise_maximum(most, __builtin_fabsf(l[i])), __builtin_fabsf(h[i]));
+    }
+    finite = most < INFINITY;
+  }
+};
+
+// sum_d max(q, 0) hi + min(q, 0) lo: q times the corner of its sign, and zero times the other
+// one, which only moves a sum where bounds are not finite (kFinite false).  The largest of kHeads heads' sums, in every lane of the block: a lane pair splits
+// the heads between them at each of the first steps, so that a step moves half of the sums of
+// the one before.
+template <int D, int kHeads, bool kFinite>
+__device__ __forceinline__ double best_of(const Query<D, kHeads>& q, const Corners& c, int lane) {
   double s[kHeads];
 #pragma unroll
   for (int h = 0; h < kHeads; ++h) {
     s[h] = 0.0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      s[h] = __builtin_fma(__builtin_fabs(q.x[h][i]), radius[i],
-                           __builtin_fma(q.x[h][i], mid[i], s[h]));
+    for (int i = 0; i < 8; ++i) {
+      const double x = q.x[h][i];
+      s[h] = __builtin_fma(x, of_upper(x < 0.0 ? c.lo[i] : c.hi[i]), s[h]);
+      if constexpr (!kFinite)
+        s[h] = __builtin_fma(0.0, of_upper(x < 0.0 ? c.hi[i] : c.lo[i]), s[h]);
+    }
   }
   double x;
   if constexpr (kHeads == 4) {
@@ -186,24 +216,26 @@ __device__ __forceinline__ void score_blocks(const SelectArgs& p, int b, int g, 
   for (int j = j0; j < end; j += step) {
     const Bounds<D> here = next;
     if (j + step < end) next.load(p, b, g, j + step + mine, part);
-    double mid[8], radius[8];
-    float lo[8], hi[8];
-    unpack8(here.lo, lo);
-    unpack8(here.hi, hi);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const double l = lo[i], h = hi[i];
-      mid[i] = h + l, radius[i] = h - l;
-    }
-    double best;
-    if constexpr (kWhole) {
-      best = best_of<D, kHeads>(q, mid, radius, lane);
-    } else {
-      best = -__builtin_inf();
+    Corners corners(here.lo, here.hi);
+    const auto best_by = [&](auto finite) {
+      if constexpr (kWhole) return best_of<D, kHeads, finite.value>(q, corners, lane);
+      double best = -__builtin_inf();
       for (int head = 0; head < p.group; head += kHeads) {
         q.load(p, b, g, head, part);
-        best = fmax(best, best_of<D, kHeads>(q, mid, radius, lane));
+        best = fmax(best, best_of<D, kHeads, finite.value>(q, corners, lane));
       }
+      return best;
+    };
+    double best;
+    if (__all(corners.finite)) {
+      best = best_by(std::true_type{});
+    } else {
+      // The rare path's own copies: corners picked for both paths ahead of the branch would be
+      // moved once more each (64 sequences of up to 32768 tokens, both launches: 34.2 us, 28.0
+      // so).
+#pragma unroll
+      for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(corners.lo[i]), "+v"(corners.hi[i]));
+      best = best_by(std::false_type{});
     }
     if (part == 0 && j + mine < end) store(j + mine, here.known ? score_key(best) : 0);
   }

@@ -9,8 +9,10 @@ if not torch.cuda.is_available():
     pytest.skip("needs an MI355X GPU", allow_module_level=True)
 
 from oracle import blocks as O
-from paged_decode.block_decode import allocate_block_resources, fp8_decode, sparse_decode
+from paged_decode.block_decode import (allocate_block_resources, fp8_decode, select_blocks,
+                                       sparse_decode)
 from paged_decode.spec import DecodeSpec
+from test_gpu_blocks import bounds_of, make, spec_of
 
 pytestmark = pytest.mark.gpu
 E4M3 = torch.float8_e4m3fn
@@ -87,3 +89,49 @@ def test_infinite_and_huge_values_of_small_weights(dim, kind):
             assert ((got[i, :, c] - exact).abs() <= allowed + 2.0 ** -8 * (abs(exact) + allowed)).all(), (s, c)
         if kind != E4M3 and i < 9:
             assert (got[i, :, 1] == math.inf).all() and (got[i, :, 2] == -math.inf).all(), s
+
+
+@pytest.mark.parametrize("power", [40, 60, None], ids=["2^40", "2^60", "lowest"])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 4, 64), (4, 2, 128), (16, 4, 256), (32, 8, 128), (9, 3, 64),
+                                      (32, 4, 256), (17, 1, 64), (40, 2, 128)])
+def test_select_by_bounds_of_any_width(hq, hkv, d, power):
+    """The corner that a query's sign leaves out moves no score, however large: a channel of
+    positive queries whose smallest keys are far below, one of negative queries whose largest
+    are far above.  With whole numbers, scores that tie."""
+    far = float(torch.finfo(torch.bfloat16).max) if power is None else 2.0 ** power
+    lengths = [64 * 300, 64 * 201 - 5, 700]
+    x = make(lengths, hq, hkv, d, torch.bfloat16, seed=hq + d)
+    gen = torch.Generator().manual_seed(hq)
+    for integers in (False, True):
+        q = (x["q"].float().round() if integers else x["q"].float())
+        q[..., 3] = q[..., 3].abs() + 1
+        q[..., d - 6] = -q[..., d - 6].abs() - 1
+        q = q.bfloat16()
+        bounds = bounds_of(x, hq + d, integers)
+        wide = torch.rand((2, *bounds.shape[:3]), generator=gen) < 0.3
+        bounds[..., 0, 3][wide[0]] = -far
+        bounds[..., 1, d - 6][wide[1]] = far
+        res = allocate_block_resources(spec_of(x), "cuda", kept=40)
+        got = select_blocks(q.cuda(), bounds.cuda(), x["tables"].cuda(), x["lengths"].cuda(),
+                            resources=res)
+        assert torch.equal(got.cpu(), O.select(q, bounds, x["tables"], x["lengths"], 40))
+
+
+def test_select_beside_bounds_that_are_not_finite():
+    """Blocks of wide, of infinite and of NaN bounds next to one another."""
+    x = make([64 * 300], 8, 2, 64, torch.bfloat16, seed=5)
+    bounds = bounds_of(x, 5)
+    gen = torch.Generator().manual_seed(5)
+    x["q"][..., 3] = x["q"][..., 3].abs() + 1
+    x["q"][0, 2, 8] = 0.0
+    wide = torch.rand(bounds.shape[:3], generator=gen) < 0.5
+    bounds[..., 0, 3][wide] = -float(torch.finfo(torch.bfloat16).max)
+    for value, corner, channel in ((math.inf, 1, 8), (-math.inf, 0, 3), (math.nan, 1, 40),
+                                   (math.nan, 0, 0)):
+        odd = torch.rand(bounds.shape[:3], generator=gen) < 0.02
+        bounds[..., corner, channel][odd] = value
+    for kept in (4, 20, 60):
+        res = allocate_block_resources(spec_of(x), "cuda", kept=kept)
+        got = select_blocks(x["q"].cuda(), bounds.cuda(), x["tables"].cuda(), x["lengths"].cuda(),
+                            resources=res)
+        assert torch.equal(got.cpu(), O.select(x["q"], bounds, x["tables"], x["lengths"], kept))
