@@ -451,7 +451,7 @@ int pd_delta_step(const float* act, const void* a, const void* b, const void* a_
  * half) or, interleaved, (2j, 2j + 1); half 0: no rotation, positions and rope
  * may be null.  q [rows, Hq, D] -> q_out (may be q); key and value -> slot
  * slot_mapping[i] of the caches, in an e4m3 cache as round(clamp(x / scale,
- * +-448)), scales positive normal numbers.  A slot outside [0, num_slots) skips
+ * +-448)), scales positive and finite.  A slot outside [0, num_slots) skips
  * the write; a position outside the table too, and the rotated part of its query
  * is NaN.  Slots of one call must differ.  Row strides are in elements, multiples of 8, heads contiguous;
  * half is a multiple of 8; num_heads may be 0.  bounds (may be null): as

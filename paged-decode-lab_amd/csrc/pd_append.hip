@@ -54,15 +54,29 @@ struct AppendArgs {
   int hq, hkv, half;
 };
 
-// x / d for a positive normal d whose reciprocal `inverse` is correctly rounded: two
-// corrections by the remainder, which an FMA gives exactly, leave the correctly rounded
-// quotient (the first is within an ulp, the second has the exact remainder of it); five
-// operations, a division is ten.  A quotient that is clamped or becomes a zero (whose sign the
-// corrections would lose), an infinity or a NaN stays as it is.
-__device__ __forceinline__ float divide(float x, float d, float inverse) {
-  const float q = x * inverse;
-  float r = __builtin_fmaf(__builtin_fmaf(-q, d, x), inverse, q);
-  r = __builtin_fmaf(__builtin_fmaf(-r, d, x), inverse, r);
+// A scale of a kv head, and the power of two that takes it into [2^-85, 2^64): there no
+// remainder of a quotient has a bit below float32's smallest number.
+struct Scale {
+  float lift, value, inverse;
+  __device__ __forceinline__ Scale(const float* scales, int head) {
+    const float d = scales ? scales[head] : 1.f;
+    lift = d < 0x1p-62f ? 0x1p64f : d > 0x1p62f ? 0x1p-64f : 1.f;
+    value = d * lift;
+    inverse = 1.f / value;
+  }
+};
+
+// x / scale, correctly rounded for positive finite scales: the reciprocal is, and two
+// corrections by the remainder, which an FMA gives exactly, leave the correctly rounded quotient
+// (the first is within an ulp, the second has the exact remainder of it); six operations, a
+// division is ten.  A quotient that is clamped or becomes a zero (whose sign the corrections
+// would lose), an infinity or a NaN stays as it is: a lifted x that overflows or loses bits is
+// one of the first two.
+__device__ __forceinline__ float divide(float x, const Scale& scale) {
+  x *= scale.lift;
+  const float q = x * scale.inverse;
+  float r = __builtin_fmaf(__builtin_fmaf(-q, scale.value, x), scale.inverse, q);
+  r = __builtin_fmaf(__builtin_fmaf(-r, scale.value, x), scale.inverse, r);
   const float size = fabsf(q);
   return size > 1e-6f && size < 1e6f ? r : q;
 }
@@ -94,18 +108,10 @@ __device__ __forceinline__ void unpack8_e4m3(u32x2_t raw, float (&x)[8]) {
   }
 }
 
-struct Scale {
-  float value, inverse;
-  __device__ __forceinline__ Scale(const float* scales, int head) {
-    value = scales ? scales[head] : 1.f;
-    inverse = 1.f / value;
-  }
-};
-
 __device__ __forceinline__ u32x2_t to_e4m3(const float (&x)[8], const Scale& scale) {
   float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = divide(x[i], scale.value, scale.inverse);
+  for (int i = 0; i < 8; ++i) y[i] = divide(x[i], scale);
   return pack8_e4m3(y);
 }
 

@@ -97,7 +97,7 @@ def append_kv(q, k, v, positions, rope, k_cache, v_cache, slot_mapping, *, inter
     ``positions`` int64 [N]: element pairs (j, j + half), or (2j, 2j + 1) with ``interleaved``,
     of the leading 2 half elements are rotated, half a multiple of 8; rope None rotates nothing.
     Caches [blocks, block_size, Hkv, D] bf16 or float8_e4m3fn, which holds x / scale (scales
-    positive normal numbers, float32 [Hkv], None: 1), clamped to +-448; ``slot_mapping`` int32
+    positive and finite, float32 [Hkv], None: 1), clamped to +-448; ``slot_mapping`` int32
     [N], a negative slot (or one past the cache) writes nothing, slots of one call must differ.
     A position outside the table writes nothing and gives its query NaN.  ``out``: where the
     queries go (q itself: in place).

@@ -2,6 +2,7 @@
 cancel, bounds of any width, scales at the ends of float32, strides of a single row."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -11,11 +12,13 @@ if not torch.cuda.is_available():
 from oracle import blocks as O
 from paged_decode.block_decode import (allocate_block_resources, fp8_decode, select_blocks,
                                        sparse_decode)
+from paged_decode.kv_append import append_kv
 from paged_decode.spec import DecodeSpec
+from test_gpu_append import bits
 from test_gpu_blocks import bounds_of, make, spec_of
 
 pytestmark = pytest.mark.gpu
-E4M3 = torch.float8_e4m3fn
+BF16, E4M3 = torch.bfloat16, torch.float8_e4m3fn
 KINDS = [torch.bfloat16, E4M3]
 IDS = ["bf16", "e4m3"]
 
@@ -135,3 +138,45 @@ def test_select_beside_bounds_that_are_not_finite():
         got = select_blocks(x["q"].cuda(), bounds.cuda(), x["tables"].cuda(), x["lengths"].cuda(),
                             resources=res)
         assert torch.equal(got.cpu(), O.select(x["q"], bounds, x["tables"], x["lengths"], kept))
+
+
+@pytest.mark.parametrize("scale", [1e-40, 2.0 ** -126, 1.1464847e-36, 1.7e-38, 3.3e-35, 1e-32, 7e-31, 1.3e-25,
+                                   2.1e-19, 5e18, 1e30, 8.6e37, 1.2e38, 3.3e38])
+def test_quotients_by_scales_of_any_size(scale):
+    """The stored value is the rounded division's, as at ordinary scales: products of the scale
+    with values and midpoints of e4m3 and the floats next to them, through a rotation by
+    (cos, 0)."""
+    n, d = 2048, 64
+    scale = torch.tensor([scale], dtype=torch.float32)
+    rng = np.random.default_rng(34)
+    grid = torch.arange(127, dtype=torch.uint8).view(E4M3).float()
+    grid = torch.cat([grid, (grid[1:] + grid[:-1]) / 2])
+    grid = grid[(grid * scale) < 1e38]
+    x = grid[torch.from_numpy(rng.integers(0, len(grid), (n, d // 2)))] * scale
+    near = torch.from_numpy(rng.integers(-2, 3, (n, d // 2)).astype(np.int32))
+    x = (x.view(torch.int32) + near * (x > 0)).view(torch.float32)
+    rope = torch.stack([x, torch.zeros_like(x)], -1).cuda()
+    k = torch.cat([torch.ones(n, 1, d // 2), torch.zeros(n, 1, d // 2)], 2).bfloat16().cuda()
+    cache = [torch.zeros((8, 256, 1, d), device="cuda").to(E4M3) for _ in range(2)]
+    at = torch.arange(n, device="cuda")
+    append_kv(None, k, k, at, rope, *cache, at.int(), k_scale=scale.cuda())
+    want = O.stored(x[:, None], scale, E4M3)
+    assert torch.equal(bits(cache[0]).view(n, d)[:, :d // 2], bits(want)[:, 0])
+
+
+@pytest.mark.parametrize("scale", [1e-42, 2.0 ** -126, 3e-37, 2.0 ** -62, 1.5 * 2.0 ** 62, 3.3e38])
+def test_special_values_by_scales_of_any_size(scale):
+    special = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0, 3.3e38, -3.3e38, 1e-38, -1e-38,
+                            1e-40, -1e-40, 2.0 ** -60, -2.0 ** 60, 1.0, -1.0, 448.0], dtype=BF16)
+    rows = special.repeat(4).view(1, 1, 64)
+    scales = torch.tensor([scale])
+    cache = [torch.zeros((1, 256, 1, 64), device="cuda").to(E4M3) for _ in range(2)]
+    append_kv(None, rows.cuda(), rows.cuda(), None, None, *cache,
+              torch.zeros(1, dtype=torch.int32, device="cuda"), k_scale=scales.cuda(),
+              v_scale=scales.cuda())
+    want = O.stored(rows.float(), scales, E4M3)[0, 0]
+    for c in cache:
+        got = c.cpu()[0, 0, 0]
+        nan = want.float().isnan()
+        assert torch.equal(got.float().isnan(), nan)
+        assert torch.equal(bits(got)[~nan], bits(want)[~nan])
