@@ -455,10 +455,10 @@ extern "C" int pd_block_bounds(const void* k_cache, int32_t cache_type, int64_t 
                                int32_t num_kv_heads, int32_t head_dim, pd_stream_t stream) {
   pd::clear_error();
   if (rows < 0) return pd::fail(PD_EINVAL, "rows must be non-negative");
-  if (!k_cache || !slot_mapping || !bounds || !all_aligned16(k_cache, bounds))
-    return pd::fail(PD_EINVAL, "tensors must be present and 16-byte aligned");
   if (const int bad = check_cache(cache_type, num_slots, bounds, num_kv_heads, head_dim)) return bad;
   if (rows == 0) return PD_OK;
+  if (!k_cache || !slot_mapping || !bounds || !all_aligned16(k_cache, bounds))
+    return pd::fail(PD_EINVAL, "tensors must be present and 16-byte aligned");
   return launch_bounds(k_cache, cache_type, num_slots, slot_mapping, rows, bounds, num_kv_heads,
                        head_dim, stream);
 }

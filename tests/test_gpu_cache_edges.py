@@ -12,7 +12,7 @@ if not torch.cuda.is_available():
 from oracle import blocks as O
 from paged_decode.block_decode import (allocate_block_resources, fp8_decode, select_blocks,
                                        sparse_decode)
-from paged_decode.kv_append import append_kv
+from paged_decode.kv_append import allocate_bounds, append_kv, block_bounds
 from paged_decode.spec import DecodeSpec
 from test_gpu_append import bits
 from test_gpu_blocks import bounds_of, make, spec_of
@@ -180,3 +180,10 @@ def test_special_values_by_scales_of_any_size(scale):
         nan = want.float().isnan()
         assert torch.equal(got.float().isnan(), nan)
         assert torch.equal(bits(got)[~nan], bits(want)[~nan])
+
+
+def test_no_rows_have_no_bounds():
+    x = torch.zeros((2, 256, 2, 64), dtype=BF16, device="cuda")
+    bounds = torch.full_like(allocate_bounds(x), 7.0)
+    block_bounds(x, torch.zeros(0, dtype=torch.int32, device="cuda"), bounds)
+    assert (bounds == 7.0).all()
