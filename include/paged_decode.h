@@ -444,7 +444,9 @@ int pd_delta_step(const float* act, const void* a, const void* b, const void* a_
 
 #define PD_BLOCK 64 /* tokens per block, four blocks a page */
 #define PD_CACHE_BF16 0
-#define PD_CACHE_E4M3 1 /* float8 e4m3fn; stored value x scale[kv head] (float32, null: 1) */
+/* float8 e4m3fn; stored value x scale[kv head] (float32, null: 1; with a bf16 cache
+ * anything but null is PD_EINVAL) */
+#define PD_CACHE_E4M3 1
 
 /* Row i: the leading 2 half elements of its query and key heads rotated by
  * rope[positions[i]] (float32 [max_positions, half, 2]: cos, sin), pairs (j, j +

@@ -404,6 +404,8 @@ extern "C" int pd_append_kv(const void* q, int64_t q_stride, const void* k, int6
   pd::clear_error();
   if (rows < 0 || num_heads < 0) return pd::fail(PD_EINVAL, "rows and heads must be non-negative");
   if (const int bad = check_cache(cache_type, num_slots, bounds, num_kv_heads, head_dim)) return bad;
+  if (cache_type == PD_CACHE_BF16 && (k_scale || v_scale))
+    return pd::fail(PD_EINVAL, "scales belong to an e4m3 cache");
   if (half < 0 || half % 8 || 2 * half > head_dim)
     return pd::fail(PD_EINVAL, "rotated pairs must be a multiple of 8, at most head_dim / 2");
   if (rows == 0) return PD_OK;

@@ -1128,6 +1128,8 @@ extern "C" int pd_block_decode(const void* q, int64_t q_stride_b, int64_t q_stri
           check_geometry(batch, num_heads, num_kv_heads, head_dim, table_width, num_pages))
     return bad;
   if (!pd::valid_cache(cache_type)) return pd::fail(PD_EINVAL, "unknown cache type");
+  if (cache_type == PD_CACHE_BF16 && (k_scale || v_scale))
+    return pd::fail(PD_EINVAL, "scales belong to an e4m3 cache");
   if (blocks && (kept < 1 || kept > 1 << 26))
     return pd::fail(PD_EINVAL, "the list must hold at least one block, at most 2^26");
   if (splits < 1 || splits > kMaxSplits)
