@@ -12,7 +12,7 @@ are not checked, nothing allocates, synchronizes or reads device memory on the h
 can be captured in a hipGraph).  Lengths past the table count as its capacity; a page outside
 the cache is read as having no tokens.  A sequence's output depends on the batch through its
 next power of two alone, so a padded graph bucket gives the bits of the eager call.
-Inference only.
+Inference only: a query, cache or bounds that ask for a gradient are refused.
 """
 from dataclasses import dataclass, field
 import math
@@ -120,6 +120,8 @@ def _attend(q, k, v, tables, lengths, blocks, resources, scale, k_scale, v_scale
     scale = dim ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise ValueError("decode attention has no gradient: call it under torch.no_grad()")
     out = resources.out
     _native.launch(device, _native.lib().pd_block_decode, q.data_ptr(), stride_b, stride_h,
                    k.data_ptr(), v.data_ptr(), cache_type, shape[0], tables.data_ptr(), table_stride,
@@ -164,6 +166,8 @@ def select_blocks(q, bounds, tables, lengths, *, resources, first=1, last=1):
     if (shape[1:] != (_PER_PAGE, hkv, 2, dim) or bounds.dtype != torch.bfloat16
             or not bounds.is_contiguous() or bounds.get_device() != device or shape[0] == 0):
         raise ValueError("bounds must be contiguous BF16 [pages, 4, kv_heads, 2, head_dim]")
+    if torch.is_grad_enabled() and (q.requires_grad or bounds.requires_grad):
+        raise ValueError("select_blocks has no gradient: call it under torch.no_grad()")
     _native.launch(device, _native.lib().pd_select_blocks, q.data_ptr(), stride_b, stride_h,
                    bounds.data_ptr(), shape[0], tables.data_ptr(), table_stride, width,
                    lengths.data_ptr(), resources.keys.data_ptr(), blocks.data_ptr(), resources.kept,

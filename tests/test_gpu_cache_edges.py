@@ -15,7 +15,7 @@ from paged_decode.block_decode import (allocate_block_resources, fp8_decode, sel
 from paged_decode.kv_append import allocate_bounds, append_kv, block_bounds
 from paged_decode.spec import DecodeSpec
 from test_gpu_append import bits
-from test_gpu_blocks import bounds_of, make, spec_of
+from test_gpu_blocks import attend, bounds_of, dev, make, spec_of
 
 pytestmark = pytest.mark.gpu
 BF16, E4M3 = torch.bfloat16, torch.float8_e4m3fn
@@ -187,3 +187,24 @@ def test_no_rows_have_no_bounds():
     bounds = torch.full_like(allocate_bounds(x), 7.0)
     block_bounds(x, torch.zeros(0, dtype=torch.int32, device="cuda"), bounds)
     assert (bounds == 7.0).all()
+
+
+def test_gradients_are_refused():
+    x = make([700, 90], 8, 2, 128, E4M3, seed=61)
+    g = dev(x)
+    dense = allocate_block_resources(spec_of(x), "cuda")
+    listed = allocate_block_resources(spec_of(x), "cuda", kept=3)
+    blocks = torch.zeros((2, 2, 3), dtype=torch.int32, device="cuda")
+    bounds = bounds_of(x, 61).cuda()
+    q = g["q"].clone().requires_grad_()
+    keys = g["k"].bfloat16().requires_grad_()
+    calls = [lambda: attend(x, dict(g, q=q), dense),
+             lambda: attend(x, dict(g, q=q), listed, blocks),
+             lambda: attend(x, dict(g, k=keys, v=g["v"].bfloat16(), k_scale=None, v_scale=None),
+                            listed, blocks),
+             lambda: select_blocks(q, bounds, g["tables"], g["lengths"], resources=listed)]
+    for call in calls:
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
