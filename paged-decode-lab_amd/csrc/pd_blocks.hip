@@ -999,6 +999,12 @@ many_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
       u32x2_t{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
 }
 
+// Strides of Q's rows that keep them 16-byte aligned; that of a dimension of one entry is not
+// used.
+bool aligned_rows(int64_t stride_b, int64_t stride_h, int32_t batch, int32_t num_heads) {
+  return (batch == 1 || stride_b % 8 == 0) && (num_heads == 1 || stride_h % 8 == 0);
+}
+
 int tile_tokens(int head_dim, int32_t cache_type) {
   return cache_type == PD_CACHE_E4M3 ? 32 : 4096 / head_dim;
 }
@@ -1036,7 +1042,7 @@ extern "C" int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_str
   if (first < 0 || last < 1 || kept < first || kept - first < last)
     return pd::fail(PD_EINVAL, "kept blocks must hold the first ones and at least one last");
   if (!q || !bounds || !table || !lengths || !keys || !blocks || !all_aligned16(q, bounds) ||
-      q_stride_b % 8 || q_stride_h % 8)
+      !aligned_rows(q_stride_b, q_stride_h, batch, num_heads))
     return pd::fail(PD_EINVAL, "tensors must be present, query rows and bounds 16-byte aligned");
   if (batch > 65535 || num_kv_heads > 65535)
     return pd::fail(PD_EINVAL, "grid dimension exceeds device limits");
@@ -1135,7 +1141,8 @@ extern "C" int pd_block_decode(const void* q, int64_t q_stride_b, int64_t q_stri
   if (splits < 1 || splits > kMaxSplits)
     return pd::fail(PD_EINVAL, "splits must be in [1, %d]", kMaxSplits);
   if (!q || !k || !v || !table || !lengths || !out || (splits > 1 && (!part_o || !part_ml)) ||
-      !all_aligned16(q, k, v, part_o, part_ml, out) || q_stride_b % 8 || q_stride_h % 8)
+      !all_aligned16(q, k, v, part_o, part_ml, out) ||
+      !aligned_rows(q_stride_b, q_stride_h, batch, num_heads))
     return pd::fail(PD_EINVAL, "tensors must be present, with 16-byte aligned rows");
   DecodeArgs p;
   p.k_scale = k_scale, p.v_scale = v_scale, p.part_o = part_o, p.part_ml = part_ml;

@@ -40,3 +40,20 @@ def test_scales_of_a_bf16_cache(scale):
         call = dict(x, cache_type=cache_type, **{scale: 64})
         assert _native.lib().pd_block_decode(*call.values()) == _native.PD_EINVAL
         assert message in _native.lib().pd_last_error()
+
+
+@pytest.mark.parametrize("batch,heads,stride_b,stride_h", [
+    (2, 8, 516, 64), (1, 8, 3, 68), (2, 1, 3, 5), (2, 8, 512, 68)])
+def test_strides_of_queries(batch, heads, stride_b, stride_h):
+    """The strides that a call uses are multiples of 8."""
+    x = dict(q=64, q_stride_b=stride_b, q_stride_h=stride_h, bounds=64, pages=9, table=64,
+             table_stride=4, width=4, lengths=64, keys=64, blocks=64, kept=3, first=1, last=1,
+             batch=batch, heads=heads, kv_heads=1, head_dim=64, stream=0)
+    assert _native.lib().pd_select_blocks(*x.values()) == _native.PD_EINVAL
+    assert b"aligned" in _native.lib().pd_last_error()
+    x = dict(q=64, q_stride_b=stride_b, q_stride_h=stride_h, k=64, v=64, cache_type=1, pages=9,
+             table=64, table_stride=4, width=4, lengths=64, blocks=64, kept=3, k_scale=0, v_scale=0,
+             part_o=64, part_ml=64, splits=2, out=64, batch=batch, heads=heads, kv_heads=1,
+             head_dim=64, scale=0.1, stream=0)
+    assert _native.lib().pd_block_decode(*x.values()) == _native.PD_EINVAL
+    assert b"aligned" in _native.lib().pd_last_error()

@@ -15,7 +15,7 @@ from paged_decode.block_decode import (allocate_block_resources, fp8_decode, sel
 from paged_decode.kv_append import allocate_bounds, append_kv, block_bounds
 from paged_decode.spec import DecodeSpec
 from test_gpu_append import bits
-from test_gpu_blocks import attend, bounds_of, dev, make, spec_of
+from test_gpu_blocks import attend, bounds_of, check, dev, make, spec_of
 
 pytestmark = pytest.mark.gpu
 BF16, E4M3 = torch.bfloat16, torch.float8_e4m3fn
@@ -208,3 +208,23 @@ def test_gradients_are_refused():
             call()
         with torch.no_grad():
             call()
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=IDS)
+@pytest.mark.parametrize("heads", [1, 4])
+def test_one_row_of_any_stride(heads, kind):
+    """A dimension of one entry has a stride that nothing reads."""
+    x = make([700], heads, 1, 128, kind, seed=62)
+    g = dev(x)
+    strides = (3, 128 if heads > 1 else 5, 1)
+    res = allocate_block_resources(spec_of(x), "cuda", kept=9)
+    blocks = torch.arange(9, dtype=torch.int32, device="cuda").view(1, 1, 9)
+    bounds = bounds_of(x, 62).cuda()
+    plain = [attend(x, g, res, blocks).clone(),
+             select_blocks(g["q"], bounds, g["tables"], g["lengths"], resources=res).clone()]
+    g["q"] = torch.as_strided(g["q"], g["q"].shape, strides)
+    assert torch.equal(attend(x, g, res, blocks), plain[0])
+    assert torch.equal(select_blocks(g["q"], bounds, g["tables"], g["lengths"], resources=res),
+                       plain[1])
+    if kind == E4M3:
+        check(attend(x, g, allocate_block_resources(spec_of(x), "cuda")), x)
