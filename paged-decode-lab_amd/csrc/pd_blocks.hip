@@ -999,6 +999,13 @@ many_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
       u32x2_t{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
 }
 
+// The next power of two: what a batch's plan depends on.
+int64_t batch_bucket(int32_t batch) {
+  int64_t rows = 1;
+  while (rows < batch) rows *= 2;
+  return rows;
+}
+
 // Strides of Q's rows that keep them 16-byte aligned; that of a dimension of one entry is not
 // used.
 bool aligned_rows(int64_t stride_b, int64_t stride_h, int32_t batch, int32_t num_heads) {
@@ -1085,13 +1092,6 @@ extern "C" int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_str
                      as_stream(stream), lengths, keys, blocks, table_width, num_kv_heads, kept,
                      first, last);
   return launch_status("pd_select_blocks");
-}
-
-// The next power of two: what a batch's plan depends on.
-int64_t batch_bucket(int32_t batch) {
-  int64_t rows = 1;
-  while (rows < batch) rows *= 2;
-  return rows;
 }
 
 extern "C" int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_heads,

@@ -1,5 +1,8 @@
 """Arguments of the cache operators at the C boundary, without a GPU: the smallest calls, and
 combinations that would be computed otherwise than they read."""
+import shutil
+import subprocess
+
 import pytest
 
 from paged_decode import _native
@@ -57,3 +60,15 @@ def test_strides_of_queries(batch, heads, stride_b, stride_h):
              head_dim=64, scale=0.1, stream=0)
     assert _native.lib().pd_block_decode(*x.values()) == _native.PD_EINVAL
     assert b"aligned" in _native.lib().pd_last_error()
+
+
+def test_the_library_exports_its_own_names_only():
+    """A function of another name could be replaced by a program's own of that name."""
+    nm = shutil.which("nm")
+    if nm is None:
+        pytest.skip("needs nm")
+    listed = subprocess.run([nm, "-D", "-C", "--defined-only", _native.lib()._name], check=True,
+                            capture_output=True, text=True).stdout
+    names = [line.split(None, 2)[2] for line in listed.splitlines() if " T " in line]
+    assert "pd_block_decode" in names
+    assert [n for n in names if not n.startswith(("pd_", "pd::"))] == []
