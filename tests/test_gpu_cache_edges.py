@@ -228,3 +228,25 @@ def test_one_row_of_any_stride(heads, kind):
                        plain[1])
     if kind == E4M3:
         check(attend(x, g, allocate_block_resources(spec_of(x), "cuda")), x)
+
+
+def test_choices_and_dense_attention_have_their_bits_in_every_batch_of_a_bucket():
+    """Five rows of eight, as a padded step has them: the rows' own bits, in every order."""
+    lengths = [700, 90, 5000, 64, 0, 3333, 1, 4097]
+    x = make(lengths, 8, 2, 128, E4M3, seed=44)
+    g = dev(x)
+    spec = DecodeSpec(8, 8, 2, 128, 5120)
+    dense = allocate_block_resources(spec, "cuda")
+    listed = allocate_block_resources(spec, "cuda", kept=9)
+    bounds = bounds_of(x, 44).cuda()
+
+    def step(rows):
+        part = {n: t[rows] if n in ("q", "tables", "lengths") else t for n, t in g.items()}
+        return (attend(x, part, dense).clone(),
+                select_blocks(part["q"], bounds, part["tables"], part["lengths"],
+                              resources=listed).clone())
+
+    whole = step(list(range(8)))
+    for rows in ([0, 1, 2, 3, 4], [7, 2, 5, 0, 4, 1], [6, 5, 4, 3, 2, 1, 0]):
+        for got, want in zip(step(rows), whole):
+            assert torch.equal(got, want[rows])
