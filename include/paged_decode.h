@@ -453,11 +453,11 @@ int pd_delta_step(const float* act, const void* a, const void* b, const void* a_
  * half) or, interleaved, (2j, 2j + 1); half 0: no rotation, positions and rope
  * may be null.  q [rows, Hq, D] -> q_out (may be q); key and value -> slot
  * slot_mapping[i] of the caches, in an e4m3 cache as round(clamp(x / scale,
- * +-448)), scales positive and finite.  A slot outside [0, num_slots) skips
- * the write; a position outside the table too, and the rotated part of its query
- * is NaN.  Slots of one call must differ.  Row strides are in elements, multiples of 8, heads contiguous;
- * half is a multiple of 8; num_heads may be 0.  bounds (may be null): as
- * pd_block_bounds, of the keys just written. */
+ * +-448)), scales positive and finite.  A slot outside [0, num_slots) skips the
+ * write; a position outside the table too, and the rotated part of its query is
+ * NaN.  Slots of one call must differ.  Row strides are in elements, multiples of
+ * 8 (of one row: any), heads contiguous; half is a multiple of 8; num_heads may be
+ * 0.  bounds (may be null): as pd_block_bounds, of the keys just written. */
 int pd_append_kv(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                  int64_t v_stride, const int64_t* positions, const float* rope,
                  int64_t max_positions, int32_t half, int32_t interleaved, void* q_out,
@@ -477,8 +477,9 @@ int pd_block_bounds(const void* k_cache, int32_t cache_type, int64_t num_slots,
  * bounds) and those of the highest scores, score = max over the group's query
  * heads of sum_d max(q, 0) high + min(q, 0) low in 64 bits, ties to the lowest
  * block; ascending, -1 behind a sequence of fewer.  A NaN score (an infinite
- * query's too) counts as +infinity, a page outside [0, num_pages) as the lowest.  keys: workspace uint64
- * [batch, Hkv, table_width * 4]. */
+ * query's too) counts as +infinity, a page outside [0, num_pages) as the lowest.
+ * keys: workspace uint64 [batch, Hkv, table_width * 4].  Here and below the strides
+ * of a dimension of one entry are not looked at. */
 int pd_select_blocks(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* bounds,
                      int64_t num_pages, const int32_t* table, int64_t table_stride_b,
                      int32_t table_width, const int32_t* lengths, uint64_t* keys, int32_t* blocks,
@@ -497,9 +498,11 @@ int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_heads, int3
  * below the length of the blocks listed for the sequence and kv head (int32
  * [batch, Hkv, kept]; null: of every block).  Entries below 0 or past the length
  * and pages outside [0, num_pages) have no tokens, an entry that is listed twice
- * counts twice, a row without tokens is 0.  With splits > 1 the blocks are cut
- * into that many spans (part_o float32 [batch, Hq, splits, D], part_ml [batch,
- * Hq, splits, 2]) and a second launch joins them. */
+ * counts twice, a row without tokens is 0.  With splits > 1 up to that many
+ * workgroups of a row take its tiles (16 to 64 tokens) in turn, as many as its
+ * length needs, and a second launch joins them.  part_o (float32 [batch, Hq,
+ * splits, D]) and part_ml ([batch, Hq, splits, 2]) are scratch: what unused splits
+ * have there is not written, nor anything for a row of one used split. */
 int pd_block_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k,
                     const void* v, int32_t cache_type, int64_t num_pages, const int32_t* table,
                     int64_t table_stride_b, int32_t table_width, const int32_t* lengths,

@@ -23,9 +23,9 @@
 // occupancy: 67 us, 49 in two launches.)
 //
 // Measured on MI355X, bounds included: those prompts (bf16, Hq 32 / Hkv 8 / D
-// 128, 209 MB) 43 + 5.6 us, 4.9 TB/s in the first launch; 2049 e4m3 rows, Hq =
-// Hkv = 16, D 64, 8 + 3.4; a decode step of 64 rows 4.8 (6.1 in two launches), of
-// one row 4.9, launch and latencies.
+// 128, 209 MB) 42.8 + 5.7 us, 4.9 TB/s in the first launch; 2049 e4m3 rows, Hq =
+// Hkv = 16, D 64, 8.4 + 4.0; a decode step of 64 rows 4.9 (6.1 in two launches),
+// of one row 4.9, launch and latencies.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -13,23 +13,29 @@
 // Attention: bound by the bytes of K and V.  Wavefronts walk the tiles of a
 // sequence (or list) with private softmax states, K and V in registers from
 // their loads to the matrix instructions, and are joined in LDS at the end of a
-// workgroup; the splits of a sequence by a second launch.  Matrix and vector
-// instructions take a quarter of the time that the bytes do (counters: 64
-// sequences of up to 32768 e4m3 tokens, Hq 32 / Hkv 8 / D 128, 24% of the SIMDs'
-// clocks), which is what the products in three bf16 terms of the probabilities
-// and the e4m3 conversions are paid from.  Measured on MI355X, both launches:
-//   64 sequences of 1 to 32768 e4m3 tokens, Hq 32 / Hkv 8 / D 128   388 us  5.5 TB/s
+// workgroup; the splits of a sequence by a second launch.  Vector instructions
+// take a third of the time that the bytes do (counters: 64 sequences of up to
+// 32768 e4m3 tokens, Hq 32 / Hkv 8 / D 128, 35% of the SIMDs' clocks), which is
+// what the products in three bf16 terms of the probabilities and the e4m3
+// conversions are paid from.  Measured on MI355X, both launches:
+//   64 sequences of 1 to 32768 e4m3 tokens, Hq 32 / Hkv 8 / D 128   391 us  5.5 TB/s
 //   128 of 1 to 4096, Hq = Hkv = 16, D 64                           124 us  4.5 TB/s
-//   64 sequences, 64 listed bf16 blocks, Hq 32 / Hkv 8 / D 128      177 us  5.5 TB/s
-//   17 sequences, 37 listed e4m3 blocks, Hq 32 / Hkv 4 / D 256     22.6 us  3.5 TB/s
-//   one, 64 listed bf16 blocks, Hq 16 / Hkv 4 / D 256               9.6 us, launches and
-//   one of 2064 e4m3 tokens, the same heads                         8.3 us  latencies
-// (a copy of 2 GiB reads and writes 4.85 TB/s).  Of the last two 6 us are the
-// attention's chain: length, table, K, softmax, join, write.
+//   64 sequences, 64 listed bf16 blocks, Hq 32 / Hkv 8 / D 128      176 us  5.6 TB/s
+//   17 sequences, 37 listed e4m3 blocks, Hq 32 / Hkv 4 / D 256     23.1 us  3.4 TB/s
+//   one, 64 listed bf16 blocks, Hq 16 / Hkv 4 / D 256              10.0 us, launches and
+//   one of 2064 e4m3 tokens, the same heads                         8.6 us  latencies
+// (a copy of 2 GiB reads and writes 4.85 TB/s; reads alone reach 6.3).  Of the
+// last two 6 to 7 us are the attention's chain: length, table, K, softmax, join,
+// write.  The bf16 decode's partition does its own chain in 4.3 us for the same
+// heads and 2064 tokens, so that one is no bound of the hardware.
 //
-// Selection: the scores are bound by their double-precision arithmetic (60% of
-// the SIMDs' clocks where the bounds' bytes would take 14 us: 64 sequences of up
-// to 32768 tokens, 21 us), the choice by its barriers (4 to 7 us).
+// Selection, by the method of ranking blocks of keys by the extremes of their
+// channels: the scores are bound by their vector instructions (57% of the SIMDs'
+// clocks where the bounds' bytes would take 14 us: 64 sequences of up to 32768
+// tokens, 22 us), the choice by its barriers (4 to 6 us).  Groups of more than
+// four heads take the query again for every run of blocks, four heads at a time:
+// 32 sequences of up to 16384 tokens, Hq 32 / Hkv 4 / D 256, 22 us where the bytes
+// take 4.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -483,7 +489,7 @@ pick_kernel(const int32_t* __restrict__ lengths, const uint64_t* __restrict__ al
 
 // Splits that a sequence of `len` tokens uses: as many as leave every wavefront a tile of it
 // (of the list, where that has fewer), or two.  The others end at once.  A table's width is a
-// capacity: 64 sequences of 500 to 1500 tokens with room for 131072 take 45 us, 34 with room
+// capacity: 64 sequences of 500 to 1500 tokens with room for 131072 take 45 us, 35 with room
 // for 1500, and 81 in as many splits as there are.
 struct SplitRule {
   int width, listed, tile, two, splits;  // listed: tiles of a list, 0: every block
@@ -1106,10 +1112,12 @@ extern "C" int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_
   const int64_t rows =
       batch_bucket(batch) * num_kv_heads * ((num_heads / num_kv_heads + 15) / 16);
   // Listed blocks are about as many for every row: one workgroup a CU, each with the most to
-  // do behind its start of some 3 us (17 rows of 37 blocks, Hq 32 / Hkv 4 / D 256, e4m3: 22.6
-  // us; 28.5 with eight).  Whole caches differ in length: eight a CU, so that no long one is
-  // left to a few (64 of 1 to 32768 tokens, Hq 32 / Hkv 8 / D 128: 387 us; 604 with two; 8 of
-  // 1000 to 9000: 23 and 25).  Nor is a long list or table: 128 tiles a workgroup at most,
+  // do behind its start of some 3 us (32 rows of 64 blocks, Hq 16 / Hkv 4 / D 256, e4m3: 53.4 us
+  // in two splits, 59.3 in three, 56.2 in four, 70.8 in one; 17 of 37 blocks, Hq 32, which fill
+  // half of their bucket: 23.5, 22.2, 23.7 and 32.8).  Whole caches differ in length: eight a
+  // CU, so that no long one is left to a few (64 of 1 to 32768 tokens, Hq 32 / Hkv 8 / D 128:
+  // 392 us, 409 with four, 506 with two; a short batch, 8 of 1000 to 9000, 24.7, 22.6 and
+  // 23.5).  Nor is a long list or table: 128 tiles a workgroup at most,
   // while the splits that short sequences leave empty are few enough (32768 workgroups).
   const int64_t groups = int64_t(listed ? 1 : 8) * cus;
   const int64_t tiles = int64_t(entries) * (kBlock / tile_tokens(head_dim, cache_type));

@@ -250,3 +250,23 @@ def test_choices_and_dense_attention_have_their_bits_in_every_batch_of_a_bucket(
     for rows in ([0, 1, 2, 3, 4], [7, 2, 5, 0, 4, 1], [6, 5, 4, 3, 2, 1, 0]):
         for got, want in zip(step(rows), whole):
             assert torch.equal(got, want[rows])
+
+
+def test_select_beside_pages_outside_the_cache():
+    """Blocks of a page that the cache does not have rank below all others, the lowest first."""
+    gen = torch.Generator().manual_seed(6)
+    bounds = torch.randn((3, 4, 1, 1, 64), generator=gen).expand(3, 4, 1, 2, 64).bfloat16()
+    q = torch.randn((2, 4, 64), generator=gen).bfloat16()
+    lengths = torch.full((2,), 64 * 12, dtype=torch.int32)
+    for outside in (-5, 3, 2 ** 31 - 1):
+        tables = torch.tensor([[0, outside, 2], [1, outside, 0]], dtype=torch.int32)
+        known = torch.tensor([[0, 1, 2], [1, 2, 0]], dtype=torch.int32)
+        for kept in (5, 8, 10):
+            res = allocate_block_resources(DecodeSpec(2, 4, 1, 64, 768), "cuda", kept=kept)
+            got = select_blocks(q.cuda(), bounds.contiguous().cuda(), tables.cuda(), lengths.cuda(),
+                                resources=res).cpu()
+            for b in range(2):
+                j = torch.tensor([i for i in range(1, 11) if not 4 <= i < 8])
+                s = O.scores(q[b], bounds[known[b, j // 4].long(), j % 4][:, 0])
+                order = j[torch.sort(s, descending=True, stable=True).indices].tolist() + [4, 5, 6, 7]
+                assert got[b, 0].tolist() == sorted([0, *order[:kept - 2], 11])
