@@ -166,9 +166,9 @@ struct Corners {
 };
 
 // sum_d max(q, 0) hi + min(q, 0) lo: q times the corner of its sign, and zero times the other
-// one, which only moves a sum where bounds are not finite (kFinite false).  The largest of kHeads heads' sums, in every lane of the block: a lane pair splits
-// the heads between them at each of the first steps, so that a step moves half of the sums of
-// the one before.
+// one, which only moves a sum where bounds are not finite (kFinite false).  The largest of
+// kHeads heads' sums, in every lane of the block: a lane pair splits the heads between them at
+// each of the first steps, so that a step moves half of the sums of the one before.
 template <int D, int kHeads, bool kFinite>
 __device__ __forceinline__ double best_of(const Query<D, kHeads>& q, const Corners& c, int lane) {
   double s[kHeads];
@@ -607,9 +607,9 @@ __device__ __forceinline__ floatx4_t mfma_pv(const Words<kPer / 2>& a, const Wor
 // cutting.  One term's error would be as large as the output's own rounding; two (16 bits) move
 // some outputs to the other side of theirs (64 sequences of up to 32768 e4m3 tokens: 1.3e-4
 // from the float32 form, relative, 2.2e-5 with three) and are hardly cheaper (398 us both; 16
-// of up to 8192, Hkv 16, D 64: 34.3 and 35.5).  Where p is not zero, neither is any of them (2^-133 at least), so that an infinite
-// V times each is that infinity: 2^-132 more than p at most, which float32 does not see for p
-// above 2^-108.
+// of up to 8192, Hkv 16, D 64: 34.3 and 35.5).  Where p is not zero, neither is any of them
+// (2^-133 at least), so that an infinite V times each is that infinity: 2^-132 more than p at
+// most, which float32 does not see for p above 2^-108.
 struct Terms {
   uint32_t hi, mid, lo;
   __device__ __forceinline__ explicit Terms(float p) {
@@ -1117,8 +1117,8 @@ extern "C" int pd_block_splits(int32_t batch, int32_t num_heads, int32_t num_kv_
   // half of their bucket: 23.5, 22.2, 23.7 and 32.8).  Whole caches differ in length: eight a
   // CU, so that no long one is left to a few (64 of 1 to 32768 tokens, Hq 32 / Hkv 8 / D 128:
   // 392 us, 409 with four, 506 with two; a short batch, 8 of 1000 to 9000, 24.7, 22.6 and
-  // 23.5).  Nor is a long list or table: 128 tiles a workgroup at most,
-  // while the splits that short sequences leave empty are few enough (32768 workgroups).
+  // 23.5).  Nor is a long list or table: 128 tiles a workgroup at most, while the splits that
+  // short sequences leave empty are few enough (32768 workgroups).
   const int64_t groups = int64_t(listed ? 1 : 8) * cus;
   const int64_t tiles = int64_t(entries) * (kBlock / tile_tokens(head_dim, cache_type));
   const int64_t want = std::max((groups + rows - 1) / rows, tiles / 128);
